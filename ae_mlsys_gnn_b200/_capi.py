@@ -108,6 +108,10 @@ PROTOTYPES = {
     "gnn_peer_close": [_PTR],
     "gnn_halo_push": [_PTR, _I64, _PTR, _PTR, _PTR, _INT, _PTR, _I64, _PTR],
     "gnn_halo_push_ranges": [_PTR, _I64, _PTR, _PTR, _PTR, _PTR, _INT, _PTR, _I64, _PTR],
+    "gnn_rms_norm_fwd": [_PTR, _PTR, _PTR, _INT, _INT, _I64, _I64, _F32, _PTR, _PTR, _PTR, _PTR],
+    "gnn_rms_norm_fp8": [_PTR, _PTR, _PTR, _INT, _INT, _I64, _I64, _F32, _INT, _PTR, _PTR, _PTR, _PTR],
+    "gnn_rms_norm_bwd_workspace_bytes": [_I64, _I64, _SZP],
+    "gnn_rms_norm_bwd": [_PTR, _PTR, _PTR, _PTR, _PTR, _INT, _INT, _I64, _I64, _PTR, _PTR, _PTR, _SZ, _PTR],
 }
 _RESTYPES = {"gnn_last_error_string": C.c_char_p}
 
@@ -171,7 +175,11 @@ KERNELS_PER_CALL = {
     "gnn_gaussian_fwd": 1, "gnn_gaussian_bwd": 2, "gnn_mhspmm": 2, "gnn_mhsddmm": 1,
     "gnn_sddmm_coo": 1, "gnn_mhtranspose": 1, "gnn_u_add_v_fwd": 1, "gnn_u_add_v_bwd": 1,
     "gnn_edge_softmax_fwd": 1, "gnn_edge_softmax_bwd": 1, "gnn_knn_graph": 1, "gnn_halo_push": 1, "gnn_halo_push_ranges": 1,
+    "gnn_rms_norm_fwd": 1, "gnn_rms_norm_fp8": 1, "gnn_rms_norm_bwd": 2,
 }
+
+# Element type codes of the feed-forward operators (GNN_F32, GNN_BF16, GNN_F16)
+DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 class CallTimer:
@@ -215,6 +223,17 @@ def call(name: str, *args) -> None:
     t.records.append((name, a, b))
 
 
+def launch(dev: torch.device, name: str, *args) -> None:
+    """``call`` on ``dev`` and its current stream, which is passed as the last argument.  The current
+    device is switched only when it is another one (small calls are bound by the host)."""
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    if dev.index == torch.cuda.current_device():
+        call(name, *args, stream)
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, stream)
+
+
 def workspace_bytes(name: str, *args) -> int:
     out = C.c_size_t(0)
     check(getattr(lib(), name)(*args, C.byref(out)), name)
@@ -246,6 +265,28 @@ def require(t: torch.Tensor, dtype: torch.dtype, name: str, ndim: int | None = N
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     return t
+
+
+def rows_of(t: torch.Tensor, name: str, width: int | None = None, like: torch.Tensor | None = None) -> torch.Tensor:
+    """Validation of a matrix of rows in one of the feed-forward types, with any number of leading
+    dimensions: CUDA device, type, last dimension; ``like``: same device, type and shape.  Rows
+    that are not laid out one after the other are copied."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (no CPU path exists)")
+    if t.dtype not in DTYPE_CODES:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if t.dim() < 1:
+        raise ValueError(f"{name} must have at least 1 dim")
+    if width is not None and t.shape[-1] != width:
+        raise ValueError(f"{name} must have {width} columns, got shape {tuple(t.shape)}")
+    if like is not None:
+        if t.device != like.device:
+            raise ValueError(f"{name} is on {t.device}, expected {like.device}")
+        if t.dtype != like.dtype:
+            raise TypeError(f"{name} must be {like.dtype}, got {t.dtype}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 _workspaces: dict[tuple[int, int], torch.Tensor] = {}

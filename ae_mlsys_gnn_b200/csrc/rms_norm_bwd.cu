@@ -1,0 +1,239 @@
+// Gradients of the root-mean-square norm.
+//
+//   u = grad_y * weight, xhat = h * rstd
+//   grad_x = rstd * (u - xhat * mean(u * xhat)) + grad_h,   grad_w = sum_rows grad_y * xhat
+//
+// One pass: grad_y, h and grad_h are read once and grad_x written once (HBM-bound).  A CTA walks
+// many rows, with the next row's loads in flight while the current one is reduced, and its threads
+// keep the weight gradient of their own columns in fp32 registers; the CTAs' sums go to a
+// workspace and a second kernel adds them in a fixed order, so the result is reproducible.
+#include <type_traits>
+#include "rms_norm.cuh"
+
+namespace gnn {
+namespace {
+
+constexpr int kBwdCtas = 148 * 4;  // partial sums of the weight gradient
+
+struct BwdParams {
+  const void* gy;
+  const void* gh;  // nullptr: none
+  const void* h;
+  const void* weight;
+  const float* rstd;
+  int w_f32;
+  int64_t n;
+  int d, group;
+  void* gx;
+  float* partial;  // [gridDim.x][d], nullptr: no weight gradient
+};
+
+// The vectors of grad_y, h and grad_h that a thread holds of one row, as they lie in memory.
+template <class T, int VEC, int NV>
+struct RowParts {
+  Pack<T, VEC> gy[NV], h[NV], gh[NV];
+  float rstd;
+};
+
+template <class T, int VEC, int NV, int MAXT>
+__global__ void __launch_bounds__(MAXT) rms_norm_bwd_kernel(const BwdParams p) {
+  __shared__ float s_sum[2][32];
+  extern __shared__ float s_gw[];  // [d], groups within one warp only
+  using P = Pack<T, VEC>;
+  // Narrow shares are requested one row ahead and keep their weights in registers; for wide ones
+  // (32 elements a thread) the registers do not suffice, and more bytes are in flight anyway.
+  constexpr bool kAhead = NV * VEC <= 16, kKeepWeight = NV * VEC <= 8;
+  const int G = p.group;
+  const int t = threadIdx.x & (G - 1), local = threadIdx.x / G;
+  const int rows = blockDim.x / G;
+  const int nvec = p.d / VEC;
+  const T* const gy = static_cast<const T*>(p.gy);
+  const T* const gh = static_cast<const T*>(p.gh);
+  const T* const h = static_cast<const T*>(p.h);
+
+  float gw[NV][VEC], wk[kKeepWeight ? NV : 1][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) gw[i][j] = 0.f;
+    if constexpr (kKeepWeight)
+      if (t + G * i < nvec) load_weight<T, VEC>(p.weight, p.w_f32, (int64_t)(t + G * i) * VEC, wk[i]);
+  }
+
+  auto request = [&](int64_t row, RowParts<T, VEC, NV>& q) {
+    if (row >= p.n) return;
+    q.rstd = p.rstd[row];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (t + G * i < nvec) {
+        const int64_t at = row * p.d + (int64_t)(t + G * i) * VEC;
+        q.gy[i] = load_pack(reinterpret_cast<const P*>(gy + at));
+        q.h[i] = load_pack(reinterpret_cast<const P*>(h + at));
+        if (gh) q.gh[i] = load_pack(reinterpret_cast<const P*>(gh + at));
+      }
+  };
+  // u = grad_y * weight, x = xhat of vector i
+  auto unpack = [&](const RowParts<T, VEC, NV>& q, int i, float (&g)[VEC], float (&u)[VEC], float (&x)[VEC]) {
+    float w[VEC];
+    q.gy[i].widen(g);
+    q.h[i].widen(x);
+    if constexpr (!kKeepWeight) load_weight<T, VEC>(p.weight, p.w_f32, (int64_t)(t + G * i) * VEC, w);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      x[j] *= q.rstd;
+      u[j] = g[j] * (kKeepWeight ? wk[kKeepWeight ? i : 0][j] : w[j]);
+    }
+  };
+
+  RowParts<T, VEC, NV> cur, next;
+  const int64_t step = (int64_t)gridDim.x * rows;
+  int64_t row = (int64_t)blockIdx.x * rows + local;
+  request(row, kAhead ? next : cur);
+  int turn = 0;
+  // every thread of the CTA makes the same number of turns: the sums below are collective
+  for (int64_t first = (int64_t)blockIdx.x * rows; first < p.n; first += step, row += step, turn ^= 1) {
+    const bool live = row < p.n;
+    if constexpr (kAhead) {
+      cur = next;
+      request(row + step, next);
+    } else if (first != (int64_t)blockIdx.x * rows) {
+      request(row, cur);
+    }
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (live && t + G * i < nvec) {
+        float g[VEC], u[VEC], x[VEC];
+        unpack(cur, i, g, u, x);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          gw[i][j] = fmaf(g[j], x[j], gw[i][j]);
+          dot = fmaf(u[j], x[j], dot);
+        }
+      }
+    const float mean = group_sum(dot, G, s_sum[turn]) / (float)p.d;
+    if (live) {
+      T* const gx = static_cast<T*>(p.gx) + row * p.d;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (t + G * i < nvec) {
+          float g[VEC], u[VEC], x[VEC];
+          unpack(cur, i, g, u, x);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            u[j] = cur.rstd * (u[j] - x[j] * mean);
+            if (gh) u[j] += to_f32(cur.gh[i].v[j]);
+          }
+          P o;
+          o.round(u);
+          store_pack(reinterpret_cast<P*>(gx) + t + G * i, o);
+        }
+    }
+  }
+
+  if (!p.partial) return;
+  float* const out = p.partial + (size_t)blockIdx.x * p.d;
+  if (rows == 1) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (t + G * i < nvec)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) out[(t + G * i) * VEC + j] = gw[i][j];
+  } else {
+    // the CTA's groups add their sums one after the other: a fixed order
+    for (int g = 0; g < rows; ++g) {
+      if (local == g) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (t + G * i < nvec)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+              float* const at = s_gw + (t + G * i) * VEC + j;
+              *at = g == 0 ? gw[i][j] : *at + gw[i][j];
+            }
+      }
+      __syncthreads();
+    }
+    for (int i = threadIdx.x; i < p.d; i += blockDim.x) out[i] = s_gw[i];
+  }
+}
+
+// grad_w[col] = sum of the CTAs' partial sums, 32 columns and 32 row strands a CTA.
+template <class W>
+__global__ void __launch_bounds__(1024) weight_grad_kernel(const float* __restrict__ partial, int parts, int d, W* out) {
+  __shared__ float s[32][33];
+  const int col = blockIdx.x * 32 + threadIdx.x;
+  float v = 0.f;
+  if (col < d)
+    for (int r = threadIdx.y; r < parts; r += 32) v += partial[(size_t)r * d + col];
+  s[threadIdx.y][threadIdx.x] = v;
+  __syncthreads();
+  v = warp_sum(s[threadIdx.x][threadIdx.y]);
+  const int c = blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x == 0 && c < d) out[c] = from_f32<W>(v);
+}
+
+NormGeom pick_bwd(int64_t d, int vec) {
+  NormGeom g = norm_geom(d, vec, norm_ept(d), 4);
+  if (g.group <= 128) {  // several rows side by side
+    g.threads = 256;
+    g.rows = g.threads / g.group;
+  }
+  return g;
+}
+
+}  // namespace
+}  // namespace gnn
+
+using namespace gnn;
+
+extern "C" int gnn_rms_norm_bwd_workspace_bytes(int64_t n, int64_t d, size_t* bytes) {
+  if (!bytes || n < 0 || d < 1) {
+    set_last_error("gnn_rms_norm_bwd_workspace_bytes: bad argument");
+    return GNN_ERR_INVALID_ARG;
+  }
+  *bytes = (size_t)(n < kBwdCtas ? n : kBwdCtas) * d * sizeof(float) + 16;
+  return GNN_OK;
+}
+
+extern "C" int gnn_rms_norm_bwd(const void* grad_y, const void* grad_h, const void* h, const void* weight,
+                                const float* rstd, int dtype, int weight_dtype, int64_t n, int64_t d, void* grad_x,
+                                void* grad_w, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  if (int rc = norm_check("gnn_rms_norm_bwd", dtype, weight_dtype, n, d)) return rc;
+  const int elt = dtype_bytes(dtype);
+  if (n == 0) {
+    if (grad_w) cudaMemsetAsync(grad_w, 0, (size_t)d * dtype_bytes(weight_dtype), stream);
+    return check_launch("gnn_rms_norm_bwd");
+  }
+  if (!grad_y || !h || !weight || !rstd || !grad_x) {
+    set_last_error("gnn_rms_norm_bwd: null pointer");
+    return GNN_ERR_INVALID_ARG;
+  }
+  size_t need = 0;
+  gnn_rms_norm_bwd_workspace_bytes(n, d, &need);
+  if (grad_w && (!workspace || workspace_bytes < need)) {
+    set_last_error("gnn_rms_norm_bwd: workspace too small");
+    return GNN_ERR_WORKSPACE;
+  }
+  const int vec = row_vec(d, elt, (uintptr_t)grad_y | (uintptr_t)grad_h | (uintptr_t)h | (uintptr_t)weight | (uintptr_t)grad_x);
+  const NormGeom g = pick_bwd(d, vec);
+  float* const partial = grad_w ? (float*)(((uintptr_t)workspace + 15) & ~(uintptr_t)15) : nullptr;
+  BwdParams p{grad_y, grad_h, h, weight, rstd, weight_dtype == GNN_F32 && dtype != GNN_F32, n, (int)d, g.group, grad_x, partial};
+  const int64_t want = (n + g.rows - 1) / g.rows;
+  const int grid = (int)(want < kBwdCtas ? want : kBwdCtas);
+  const size_t smem = g.rows > 1 ? (size_t)d * sizeof(float) : 0;
+  dispatch_norm(dtype, vec, g.ept, [&](auto tag, auto v, auto nv) {
+    using T = decltype(tag);
+    constexpr int V = decltype(v)::value, NV = decltype(nv)::value;
+    if (g.threads <= 512) rms_norm_bwd_kernel<T, V, NV, 512><<<grid, g.threads, smem, stream>>>(p);
+    else if constexpr (V * NV == 32) rms_norm_bwd_kernel<T, V, NV, 1024><<<grid, g.threads, smem, stream>>>(p);
+  });
+  if (grad_w) {
+    const dim3 block(32, 32);
+    const unsigned cols = (unsigned)((d + 31) / 32);
+    if (weight_dtype == GNN_F32) weight_grad_kernel<<<cols, block, 0, stream>>>(partial, grid, (int)d, (float*)grad_w);
+    else if (weight_dtype == GNN_BF16) weight_grad_kernel<<<cols, block, 0, stream>>>(partial, grid, (int)d, (__nv_bfloat16*)grad_w);
+    else weight_grad_kernel<<<cols, block, 0, stream>>>(partial, grid, (int)d, (__half*)grad_w);
+  }
+  return check_launch("gnn_rms_norm_bwd");
+}

@@ -452,6 +452,36 @@ int gnn_halo_push_ranges(const float* x, int64_t row_floats, const int* send_idx
                          const int64_t* send_beg, const int64_t* send_cnt, float* const* dst,
                          int world, float* own_dst, int64_t n_own, cudaStream_t stream);
 
+/* ---- feed-forward operators (no counterpart in the reference) -------------------------------
+ * Element types of the arrays marked `dtype`: */
+#define GNN_F32 0
+#define GNN_BF16 1
+#define GNN_F16 2
+
+/* Root-mean-square norm of n rows of d elements (1 <= d <= 32768) with the residual's addition:
+ *   h = x + residual (NULL: h = x),  rstd = 1 / sqrt(mean(h^2) + eps),  y = h * rstd * weight
+ * weight [d] is of the rows' type or fp32.  y is formed from the unrounded fp32 h.  h [n,d] and
+ * rstd [n] may be NULL (not stored). */
+int gnn_rms_norm_fwd(const void* x, const void* residual, const void* weight, int dtype, int weight_dtype,
+                     int64_t n, int64_t d, float eps, void* y, void* h, float* rstd, cudaStream_t stream);
+
+/* The same norm with y stored as e4m3: scale = max(amax |y| / 448, 2^-126) over the row (block = 0,
+ * scale [n]) or over every 128 columns (block = 128, scale [n, ceil(d/128)]), q = e4m3(y / scale).
+ * A NaN in a row (block) makes its scale and values NaN. */
+int gnn_rms_norm_fp8(const void* x, const void* residual, const void* weight, int dtype, int weight_dtype,
+                     int64_t n, int64_t d, float eps, int block, void* q /*[n,d]*/, float* scale, void* h,
+                     cudaStream_t stream);
+
+/* Gradients of gnn_rms_norm_fwd from its h and rstd, u = grad_y * weight, xhat = h * rstd:
+ *   grad_x = rstd * (u - xhat * mean(u * xhat)) + grad_h     (also the residual's gradient)
+ *   grad_w = sum over rows of grad_y * xhat                  (fp32 sums in a fixed order)
+ * grad_h (NULL: none) is the gradient that reaches h itself; grad_w (NULL: not wanted) has the
+ * weight's type. */
+int gnn_rms_norm_bwd_workspace_bytes(int64_t n, int64_t d, size_t* bytes);
+int gnn_rms_norm_bwd(const void* grad_y, const void* grad_h, const void* h, const void* weight, const float* rstd,
+                     int dtype, int weight_dtype, int64_t n, int64_t d, void* grad_x, void* grad_w, void* workspace,
+                     size_t workspace_bytes, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
