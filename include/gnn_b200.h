@@ -482,6 +482,30 @@ int gnn_rms_norm_bwd(const void* grad_y, const void* grad_h, const void* h, cons
                      int dtype, int weight_dtype, int64_t n, int64_t d, void* grad_x, void* grad_w, void* workspace,
                      size_t workspace_bytes, cudaStream_t stream);
 
+/* Rows between token order and expert order.  Every token has k choices (pairs, numbered t*k + j);
+ * a pair whose expert is not one of 0..n_experts-1 (a padding token's -1) goes nowhere.
+ * gnn_expert_sort: stable counting sort of the pairs by expert.  offsets [n_experts+1]: first row
+ *   of every expert in the sorted order, offsets[n_experts] = rows in use; slots [pairs]: the pair's
+ *   row, -1 for a pair that goes nowhere.  At most 1024 experts, pairs < 2^31.
+ * gnn_expert_dispatch: out[slots[t,j]] = x[t], out [tokens*k, width].  `kept` is a device pointer to
+ *   the number of rows in use (offsets + n_experts); the rows behind them are set to zero.
+ * gnn_expert_combine: out[t] = sum_j weights[t,j] * rows[slots[t,j]] (fp32 sums in the order of j;
+ *   weights NULL: unit weights, which is the gradient of gnn_expert_dispatch).  weights are of the
+ *   rows' type or fp32.  k <= 32.
+ * gnn_expert_combine_bwd: grad_rows[slots[t,j]] = weights[t,j] * grad_out[t] (unused rows zero),
+ *   grad_weights[t,j] = <grad_out[t], rows[slots[t,j]]> (NULL: not wanted; 0 for a pair that goes
+ *   nowhere). */
+int gnn_expert_sort_workspace_bytes(int64_t pairs, int n_experts, size_t* bytes);
+int gnn_expert_sort(const void* ids, int ids_are_64_bit, int64_t pairs, int n_experts, int* offsets, int* slots,
+                    void* workspace, size_t workspace_bytes, cudaStream_t stream);
+int gnn_expert_dispatch(const void* x, const int* slots, const int* kept, int dtype, int64_t tokens, int k,
+                        int64_t width, void* out, cudaStream_t stream);
+int gnn_expert_combine(const void* rows, const void* weights, const int* slots, int dtype, int weight_dtype,
+                       int64_t tokens, int k, int64_t width, void* out, cudaStream_t stream);
+int gnn_expert_combine_bwd(const void* grad_out, const void* rows, const void* weights, const int* slots,
+                           const int* kept, int dtype, int weight_dtype, int64_t tokens, int k, int64_t width,
+                           void* grad_rows, void* grad_weights, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
