@@ -34,6 +34,7 @@
 #include <stdlib.h>
 #include "../../include/gnn_b200.h"
 #include "common.cuh"
+#include "activation.cuh"
 #include "gemm_persistent.cuh"
 
 namespace gnn {
@@ -42,27 +43,33 @@ namespace {
 constexpr int BM = 128, BK = 32;
 constexpr int kTileBytes = BM * BK * 4;      // 16 KB: one 128-row operand tile (raw/hi or lo)
 constexpr int kConvThreads = 128;
-constexpr int kThreads = 32 * 10;
+// Epilogue warps: 4, or 8 (two per 32 rows, alternate column chunks) for the linear layers, whose
+// sums leave tensor memory often and whose epilogue computes.
+template <bool FINISH>
+struct Roles {
+  static constexpr int kEpiWarps = FINISH ? 8 : 4;
+  static constexpr int kThreads = 32 * (6 + kEpiWarps);
+  // a 32 x 32 fp32 block per epilogue warp (4 KB), through which the rows a thread holds are turned
+  // into stores that cover whole 128-byte lines
+  static constexpr int kStageBytes = kEpiWarps * 32 * 32 * 4;
+};
 constexpr int kAccBufs = 2;
 constexpr int kMaxStages = 3;
 constexpr int kNumBars = 3 * kMaxStages + 2 * kAccBufs;
-// Epilogue staging: a 32 x 32 fp32 block per epilogue warp (4 KB), through which the rows a
-// thread holds are turned into stores that cover whole 128-byte lines.
-constexpr int kEpiStageBytes = 4 * 32 * 32 * 4;
 constexpr int kEpiStageOffset = (8 * kNumBars + 16 + 127) / 128 * 128;  // after the barriers and the TMEM slot, 128-byte aligned
 
 // Geometry of one instantiation.  BN = 128: three stages, 256 tensor-memory columns, any operand
 // mode.  BN = 256 (B given as split hi/lo, K-major: the projection weights): the B tile is
 // 256 rows, two stages of 96 KB, all 512 tensor-memory columns; per multiply-add it reads 2/3 of
 // the shared-memory bytes of the 128-wide tile, which is what bounds this kernel.
-template <int BN>
+template <int BN, bool FINISH = false>
 struct Geom {
   static constexpr int kStages = BN == 128 ? 3 : 2;
   static constexpr int kBTileBytes = BN * BK * 4;
   static constexpr int kStageBytes = 2 * kTileBytes + 2 * kBTileBytes;  // A0, A1, B0, B1
   static constexpr int kTmemCols = kAccBufs * BN;
   static constexpr size_t kSmemBytes =
-      (size_t)kStages * kStageBytes + 1024 /*alignment slack*/ + kEpiStageOffset + kEpiStageBytes;
+      (size_t)kStages * kStageBytes + 1024 /*alignment slack*/ + kEpiStageOffset + Roles<FINISH>::kStageBytes;
 };
 // The tensor core adds into its fp32 accumulator with truncation: a chain of n MMAs comes
 // out low by about n * 2^-26 of its value (measured: -4e-4 after 25,000 MMAs).  After this
@@ -93,6 +100,7 @@ struct Params {
   float* score_l;
   float* score_r;
   int heads, head_w;
+  GemmFinish fin;  // read by the FINISH instantiation only
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -240,15 +248,26 @@ __device__ __forceinline__ TileCoord decode_tile(const Params& p, int tile) {
   return t;
 }
 
-template <int BN>
-__global__ void __launch_bounds__(kThreads, 1)
+// The epilogue of one element at offset `at` of C.
+__device__ __forceinline__ float finish_one(const GemmFinish& f, int64_t at, int col, float v) {
+  if (f.bias) v += __ldg(f.bias + col);
+  if (f.z) f.z[at] = v;
+  v = act_value<true>(v, f.act, f.slope);
+  if (f.residual) v += __ldg(f.residual + at);
+  return v;
+}
+
+// FINISH: the epilogue of a linear layer (GemmFinish).  An instantiation of its own, so that the
+// plain product's epilogue keeps its registers.
+template <int BN, bool FINISH>
+__global__ void __launch_bounds__(Roles<FINISH>::kThreads, 1)
 gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_a1,
                        const __grid_constant__ CUtensorMap map_b0, const __grid_constant__ CUtensorMap map_b1,
                        Params p) {
-  constexpr int kStages = Geom<BN>::kStages;
-  constexpr int kStageBytes = Geom<BN>::kStageBytes;
-  constexpr int kBTileBytes = Geom<BN>::kBTileBytes;
-  constexpr int kTmemCols = Geom<BN>::kTmemCols;
+  constexpr int kStages = Geom<BN, FINISH>::kStages;
+  constexpr int kStageBytes = Geom<BN, FINISH>::kStageBytes;
+  constexpr int kBTileBytes = Geom<BN, FINISH>::kBTileBytes;
+  constexpr int kTmemCols = Geom<BN, FINISH>::kTmemCols;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t base = (raw_addr + 1023u) & ~1023u;  // swizzle atoms need 1024-byte alignment
@@ -275,7 +294,7 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_
     }
     for (int b = 0; b < kAccBufs; ++b) {
       mbar_init(acc_full_bar(b), 1);
-      mbar_init(acc_empty_bar(b), 4);
+      mbar_init(acc_empty_bar(b), Roles<FINISH>::kEpiWarps);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -374,6 +393,8 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_
   } else {
     // ---------------------------------------------------------------- epilogue
     const int lg = warp & 3;  // this warp may touch tensor-memory lanes [32*lg, 32*lg + 32)
+    constexpr int kShare = Roles<FINISH>::kEpiWarps / 4;  // warps that divide a row's column chunks
+    const int part = kShare > 1 ? (warp - 6) >> 2 : 0;
     uint32_t tcount = 0;
     bool ok = true;
     for (int tile = blockIdx.x; tile < p.num_tiles && ok && !s_failed; tile += gridDim.x) {
@@ -382,7 +403,7 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_
       float* const Cout = p.C + (size_t)t.z * p.split_stride;
       // running fp32 sum of this thread's output row when the tile has several chains (the
       // 256-wide tile is only launched for reductions that fit one chain)
-      float sum[BN == 128 ? BN : 1];
+      float sum[BN == 128 ? BN / kShare : 1];
       float dl = 0.f, dr = 0.f;  // running dot products of the current head with attn_l / attn_r
       for (int ch = 0; ch < t.chains; ++ch, ++tcount) {
         const int buf = tcount & 1;
@@ -390,11 +411,11 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const bool last = ch == t.chains - 1;
 #pragma unroll
-        for (int c = 0; c < BN / 32; ++c) {
-          const int col0 = t.n0 + c * 32;
+        for (int c = 0; c < BN / 32 / kShare; ++c) {
+          const int chunk = (c * kShare + part) * 32, col0 = t.n0 + chunk;
           if (col0 >= p.N) break;
           uint32_t r[32];
-          const uint32_t taddr = tmem_base + ((uint32_t)(lg * 32) << 16) + (uint32_t)(buf * BN + c * 32);
+          const uint32_t taddr = tmem_base + ((uint32_t)(lg * 32) << 16) + (uint32_t)(buf * BN + chunk);
           asm volatile(
               "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
               "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -419,7 +440,7 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_
               }
             }
           }
-          if (last && p.score_l != nullptr) {
+          if (!FINISH && last && p.score_l != nullptr) {
             const int ncols = min(32, p.N - col0);
             if (ncols == 32) {
 #pragma unroll
@@ -454,9 +475,11 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_
           // outputs go through the warp's staging block instead (written row-wise with the
           // 16-byte units of row r rotated by r mod 8, read back four rows at a time, both
           // conflict-free): every store instruction then covers four whole 128-byte lines.
-          const bool staged = last && p.N - col0 >= 32 && (p.ldc & 3) == 0 && ((uintptr_t)Cout & 15) == 0;  // warp-uniform
+          bool staged = last && p.N - col0 >= 32 && (p.ldc & 3) == 0 && ((uintptr_t)Cout & 15) == 0;  // warp-uniform
+          if constexpr (FINISH)
+            staged = staged && (((uintptr_t)p.fin.bias | (uintptr_t)p.fin.z | (uintptr_t)p.fin.residual) & 15) == 0;
           if (staged) {
-            float4* const stg = epi_stage + lg * 256;
+            float4* const stg = epi_stage + (lg + 4 * part) * 256;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
               stg[lane * 8 + (j ^ (lane & 7))] =
@@ -464,17 +487,64 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_
                               __uint_as_float(r[4 * j + 3]));
             __syncwarp();
             const int u = lane & 7;
+            if constexpr (FINISH) {
+              const int sub = lane >> 3;
+              const int64_t at0 = (int64_t)(t.m0 + lg * 32 + sub) * p.ldc + col0 + u * 4;  // row i: + 4 i ldc
+              const int left = p.M - (t.m0 + lg * 32 + sub);                               // row i exists: 4 i < left
+              const GemmFinish& f = p.fin;
+              float v[32];
+              float4 res[8], b = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (f.bias) b = __ldg(reinterpret_cast<const float4*>(f.bias + col0 + u * 4));
+              if (f.residual) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int rr = i * 4 + (lane >> 3);
-              const float4 v = stg[rr * 8 + (u ^ (rr & 7))];
-              const int grow = t.m0 + lg * 32 + rr;
-              if (grow < p.M) *reinterpret_cast<float4*>(Cout + (size_t)grow * p.ldc + col0 + u * 4) = v;
+                for (int i = 0; i < 8; ++i)
+                  if (4 * i < left) res[i] = __ldg(reinterpret_cast<const float4*>(f.residual + at0 + 4 * i * p.ldc));
+              }
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int rr = i * 4 + sub;
+                const float4 q = stg[rr * 8 + (u ^ (rr & 7))];
+                v[4 * i] = q.x + b.x; v[4 * i + 1] = q.y + b.y; v[4 * i + 2] = q.z + b.z; v[4 * i + 3] = q.w + b.w;
+              }
+              if (f.z) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  if (4 * i < left)
+                    *reinterpret_cast<float4*>(f.z + at0 + 4 * i * p.ldc) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+              }
+              apply_act<true>(v, f.act, f.slope);
+              if (f.residual) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  v[4 * i] += res[i].x; v[4 * i + 1] += res[i].y; v[4 * i + 2] += res[i].z; v[4 * i + 3] += res[i].w;
+                }
+              }
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (4 * i < left)
+                  *reinterpret_cast<float4*>(Cout + at0 + 4 * i * p.ldc) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int rr = i * 4 + (lane >> 3);
+                const float4 v = stg[rr * 8 + (u ^ (rr & 7))];
+                const int grow = t.m0 + lg * 32 + rr;
+                if (grow < p.M) *reinterpret_cast<float4*>(Cout + (size_t)grow * p.ldc + col0 + u * 4) = v;
+              }
             }
             __syncwarp();  // the block is rewritten by the next chunk
           } else if (last && row < p.M) {
             float* crow = Cout + (size_t)row * p.ldc + col0;
             const int ncols = min(32, p.N - col0);
+            if constexpr (FINISH) {
+              // one element at a time, for rows that are not whole 16-byte units
+              float* const mine = reinterpret_cast<float*>(epi_stage + (lg + 4 * part) * 256) + lane;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) mine[j * 32] = __uint_as_float(r[j]);
+#pragma unroll 1
+              for (int j = 0; j < ncols; ++j)
+                crow[j] = finish_one(p.fin, (int64_t)row * p.ldc + col0 + j, col0 + j, mine[j * 32]);
+            } else
             if (ncols == 32 && ((uintptr_t)crow & 15) == 0) {
 #pragma unroll
               for (int j = 0; j < 32; j += 4)
@@ -587,7 +657,7 @@ bool encode_operand(const GemmOperand& o, int64_t K, CUtensorMap* m0, CUtensorMa
   return false;
 }
 
-template <int BN>
+template <int BN, bool FINISH>
 int launch_instance(const CUtensorMap& ma0, const CUtensorMap& ma1, const CUtensorMap& mb0, const CUtensorMap& mb1,
                     Params p, int64_t b_rows, int splits, cudaStream_t stream) {
   static bool attr_set = false;  // per process and instantiation; the attribute is per device
@@ -595,8 +665,8 @@ int launch_instance(const CUtensorMap& ma0, const CUtensorMap& ma1, const CUtens
   int dev = 0;
   cudaGetDevice(&dev);
   if (!attr_set || attr_dev != dev) {
-    if (cudaFuncSetAttribute(gemm_persistent_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)Geom<BN>::kSmemBytes) != cudaSuccess) {
+    if (cudaFuncSetAttribute(gemm_persistent_kernel<BN, FINISH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)Geom<BN, FINISH>::kSmemBytes) != cudaSuccess) {
       set_last_error("gnn_gemm_tf32x3: cannot reserve dynamic shared memory");
       return GNN_ERR_CUDA;
     }
@@ -614,7 +684,7 @@ int launch_instance(const CUtensorMap& ma0, const CUtensorMap& ma1, const CUtens
   }
   p.num_tiles = (int)tiles;
   const int grid = (int)(tiles < sms ? tiles : sms);
-  gemm_persistent_kernel<BN><<<grid, kThreads, Geom<BN>::kSmemBytes, stream>>>(ma0, ma1, mb0, mb1, p);
+  gemm_persistent_kernel<BN, FINISH><<<grid, Roles<FINISH>::kThreads, Geom<BN, FINISH>::kSmemBytes, stream>>>(ma0, ma1, mb0, mb1, p);
   return GNN_OK;
 }
 
@@ -622,8 +692,8 @@ int launch_instance(const CUtensorMap& ma0, const CUtensorMap& ma1, const CUtens
 
 int launch_gemm_persistent(const GemmOperand& a, const GemmOperand& b, int64_t K, float* C, int64_t ldc,
                            int splits, int64_t split_stride, int* status, cudaStream_t stream,
-                           const GemmScores* scores) {
-  Params p;
+                           const GemmScores* scores, const GemmFinish* finish, int chain_kb) {
+  Params p = {};
   p.M = (int)a.rows;
   p.N = (int)b.rows;
   p.total_kb = (int)((K + BK - 1) / BK);
@@ -637,7 +707,7 @@ int launch_gemm_persistent(const GemmOperand& a, const GemmOperand& b, int64_t K
   p.status = status;
   p.a_mode = a.mode;
   p.b_mode = b.mode;
-  p.chain_kb = kChainKb;
+  p.chain_kb = chain_kb > 0 ? chain_kb : kChainKb;
   p.attn_l = p.attn_r = nullptr;
   p.score_l = p.score_r = nullptr;
   p.heads = 1;
@@ -654,14 +724,18 @@ int launch_gemm_persistent(const GemmOperand& a, const GemmOperand& b, int64_t K
     return !(e && e[0] == '1' && e[1] == '2' && e[2] == '8');
   }();
   const bool wide = wide_ok && b.mode == kKMajorSplit && a.mode == kKMajorRaw && splits == 1 && b.rows >= 256 &&
-                    p.total_kb <= kChainKb;
+                    p.total_kb <= p.chain_kb && !finish;
   CUtensorMap ma0, ma1, mb0, mb1;
   if (!encode_operand(a, K, &ma0, &ma1) || !encode_operand(b, K, &mb0, &mb1, wide ? 256 : BM)) {
     set_last_error("gnn_gemm_tf32x3: cuTensorMapEncodeTiled failed");
     return GNN_ERR_CUDA;
   }
-  return wide ? launch_instance<256>(ma0, ma1, mb0, mb1, p, b.rows, splits, stream)
-              : launch_instance<128>(ma0, ma1, mb0, mb1, p, b.rows, splits, stream);
+  if (finish) {
+    p.fin = *finish;
+    return launch_instance<128, true>(ma0, ma1, mb0, mb1, p, b.rows, splits, stream);
+  }
+  return wide ? launch_instance<256, false>(ma0, ma1, mb0, mb1, p, b.rows, splits, stream)
+              : launch_instance<128, false>(ma0, ma1, mb0, mb1, p, b.rows, splits, stream);
 }
 
 }  // namespace gnn

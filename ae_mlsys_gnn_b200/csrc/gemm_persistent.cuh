@@ -35,6 +35,17 @@ struct GemmScores {
   int heads, head_w;
 };
 
+// Bias, activation and residual in the epilogue (splits == 1): with v the sum at (m, n),
+//   v += bias[n];  z[m,n] = v;  v = act(v);  v += residual[m,n]        (null pointers, act 0: nothing)
+// bias is [N], z and residual have C's layout.  With splits > 1 every member is null and act 0.
+struct GemmFinish {
+  const float* bias;
+  float* z;
+  int act;
+  float slope;
+  const float* residual;
+};
+
 // Shapes for which the epilogue can form the scores: every head inside one 128-column tile and
 // starting on a 32-column chunk.
 inline bool gemm_scores_ok(int heads, int head_w) {
@@ -42,10 +53,19 @@ inline bool gemm_scores_ok(int heads, int head_w) {
 }
 
 // C[z][M][N] (z < splits) = sum over the z-th range of K blocks of A * B^T.
+// chain_kb: K blocks accumulated in tensor memory before the sum moves to registers (0: the default).
 // Returns 0, or a negative GNN_ERR_* after set_last_error.
 int launch_gemm_persistent(const GemmOperand& a, const GemmOperand& b, int64_t K, float* C, int64_t ldc,
                            int splits, int64_t split_stride, int* status, cudaStream_t stream,
-                           const GemmScores* scores = nullptr);
+                           const GemmScores* scores = nullptr, const GemmFinish* finish = nullptr, int chain_kb = 0);
+
+// gnn_gemm_tf32x3 and gnn_gemm_tf32x3_tn (gemm_tf32x3.cu) with a linear layer's epilogue and a
+// chain length of choice; `what` names the entry point in error messages.
+int tf32x3_product(const float* A, const float* B, int b_is_n_by_k, float* C, int64_t M, int64_t N, int64_t K,
+                   void* workspace, size_t workspace_bytes, int* status, cudaStream_t stream, const GemmScores* scores,
+                   const GemmFinish* finish, int chain_kb, const char* what);
+int tf32x3_product_tn(const float* A, const float* B, float* C, int64_t M, int64_t K1, int64_t N1, void* workspace,
+                      size_t workspace_bytes, int* status, cudaStream_t stream, int chain_kb);
 
 // Whether an operand with `cols` contiguous floats per row and base pointer p can be read by TMA.
 inline bool tma_rows_ok(const void* p, int64_t cols) {

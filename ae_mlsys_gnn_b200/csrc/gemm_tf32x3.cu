@@ -131,6 +131,44 @@ size_t tn_prepass_bytes(int64_t M, int64_t cols) {
 
 }  // namespace
 
+namespace gnn {
+
+int tf32x3_product(const float* A, const float* B, int b_is_n_by_k, float* C, int64_t M, int64_t N, int64_t K,
+                   void* workspace, size_t workspace_bytes, int* status, cudaStream_t stream, const GemmScores* scores,
+                   const GemmFinish* finish, int chain_kb, const char* what) {
+  if (M < 0 || N < 0 || K < 0) return bad("gnn_gemm_tf32x3: negative size");
+  if (M == 0 || N == 0) return GNN_OK;
+  if (!A || !B || !C || !status) return bad("gnn_gemm_tf32x3: null pointer");
+  if (!gnn_gemm_tf32x3_supported(M, N, K) || !tma_rows_ok(A, K)) {
+    set_last_error("gnn_gemm_tf32x3: K must be a multiple of 4 and A 16-byte aligned");
+    return GNN_ERR_UNSUPPORTED;
+  }
+  size_t need = 0;
+  gnn_gemm_tf32x3_workspace_bytes(M, N, K, &need);
+  if (!workspace || workspace_bytes < need) {
+    set_last_error("gnn_gemm_tf32x3: workspace too small");
+    return GNN_ERR_WORKSPACE;
+  }
+  char* w = (char*)align_up((uintptr_t)workspace, 256);
+  const size_t bb = align_up((size_t)N * K * 4, 256);
+  float* b_hi = (float*)w;
+  float* b_lo = (float*)(w + bb);
+  if (b_is_n_by_k) {
+    const int64_t nb = N * K;
+    split_kernel<<<(unsigned)((nb / 4 + 256) / 256), 256, 0, stream>>>(B, nb, b_hi, b_lo);
+  } else {
+    dim3 grid((unsigned)((K + 31) / 32), (unsigned)((N + 31) / 32));
+    split_transpose_kernel<<<grid, dim3(32, 8), 0, stream>>>(B, K, (int)N, K, b_hi, b_lo);
+  }
+  const GemmOperand oa{kKMajorRaw, A, nullptr, M};
+  const GemmOperand ob{kKMajorSplit, b_hi, b_lo, N};
+  const int rc = launch_gemm_persistent(oa, ob, K, C, N, 1, 0, status, stream, scores, finish, chain_kb);
+  if (rc != GNN_OK) return rc;
+  return check_launch(what);
+}
+
+}  // namespace gnn
+
 extern "C" int gnn_gemm_tf32x3_supported(int64_t M, int64_t N, int64_t K) {
   return M > 0 && N > 0 && K > 0 && K % 4 == 0 && M < (1LL << 31) && N < (1LL << 31) && K < (1LL << 31);
 }
@@ -166,36 +204,9 @@ extern "C" int gnn_gemm_tf32x3_scores(const float* A, const float* B, int b_is_n
       return GNN_ERR_UNSUPPORTED;
     }
   }
-  if (M < 0 || N < 0 || K < 0) return bad("gnn_gemm_tf32x3: negative size");
-  if (M == 0 || N == 0) return GNN_OK;
-  if (!A || !B || !C || !status) return bad("gnn_gemm_tf32x3: null pointer");
-  if (!gnn_gemm_tf32x3_supported(M, N, K) || !tma_rows_ok(A, K)) {
-    set_last_error("gnn_gemm_tf32x3: K must be a multiple of 4 and A 16-byte aligned");
-    return GNN_ERR_UNSUPPORTED;
-  }
-  size_t need = 0;
-  gnn_gemm_tf32x3_workspace_bytes(M, N, K, &need);
-  if (!workspace || workspace_bytes < need) {
-    set_last_error("gnn_gemm_tf32x3: workspace too small");
-    return GNN_ERR_WORKSPACE;
-  }
-  char* w = (char*)align_up((uintptr_t)workspace, 256);
-  const size_t bb = align_up((size_t)N * K * 4, 256);
-  float* b_hi = (float*)w;
-  float* b_lo = (float*)(w + bb);
-  if (b_is_n_by_k) {
-    const int64_t nb = N * K;
-    split_kernel<<<(unsigned)((nb / 4 + 256) / 256), 256, 0, stream>>>(B, nb, b_hi, b_lo);
-  } else {
-    dim3 grid((unsigned)((K + 31) / 32), (unsigned)((N + 31) / 32));
-    split_transpose_kernel<<<grid, dim3(32, 8), 0, stream>>>(B, K, (int)N, K, b_hi, b_lo);
-  }
-  const GemmOperand oa{kKMajorRaw, A, nullptr, M};
-  const GemmOperand ob{kKMajorSplit, b_hi, b_lo, N};
   const GemmScores sc{attn_l, attn_r, score_l, score_r, heads, head_w};
-  const int rc = launch_gemm_persistent(oa, ob, K, C, N, 1, 0, status, stream, with_scores ? &sc : nullptr);
-  if (rc != GNN_OK) return rc;
-  return check_launch("gnn_gemm_tf32x3");
+  return tf32x3_product(A, B, b_is_n_by_k, C, M, N, K, workspace, workspace_bytes, status, stream,
+                        with_scores ? &sc : nullptr, nullptr, 0, "gnn_gemm_tf32x3");
 }
 
 extern "C" int gnn_gemm_tf32x3_tn_workspace_bytes(int64_t M, int64_t K1, int64_t N1, size_t* bytes) {
@@ -208,6 +219,11 @@ extern "C" int gnn_gemm_tf32x3_tn_workspace_bytes(int64_t M, int64_t K1, int64_t
 extern "C" int gnn_gemm_tf32x3_tn(const float* A, const float* B, float* C, int64_t M, int64_t K1,
                                   int64_t N1, void* workspace, size_t workspace_bytes, int* status,
                                   cudaStream_t stream) {
+  return tf32x3_product_tn(A, B, C, M, K1, N1, workspace, workspace_bytes, status, stream, 0);
+}
+
+int gnn::tf32x3_product_tn(const float* A, const float* B, float* C, int64_t M, int64_t K1, int64_t N1, void* workspace,
+                           size_t workspace_bytes, int* status, cudaStream_t stream, int chain_kb) {
   if (M < 0 || K1 < 0 || N1 < 0) return bad("gnn_gemm_tf32x3_tn: negative size");
   if (K1 == 0 || N1 == 0) return GNN_OK;
   if (!C || !status || (M && (!A || !B))) return bad("gnn_gemm_tf32x3_tn: null pointer");
@@ -247,7 +263,9 @@ extern "C" int gnn_gemm_tf32x3_tn(const float* A, const float* B, float* C, int6
     ob = GemmOperand{kKMajorSplitBlocked, hi, lo, N1};
   }
   const int splits = tn_splits(K1, N1, M);
-  const int rc = launch_gemm_persistent(oa, ob, M, partial, N1, splits, K1 * N1, status, stream);
+  const GemmFinish plain{};  // a chain length of choice runs on the kernel of the linear layers
+  const int rc = launch_gemm_persistent(oa, ob, M, partial, N1, splits, K1 * N1, status, stream, nullptr,
+                                        chain_kb ? &plain : nullptr, chain_kb);
   if (rc != GNN_OK) return rc;
   const int64_t count = K1 * N1;
   splitk_reduce_kernel<<<(unsigned)((count + 255) / 256), 256, 0, stream>>>(partial, splits, count, C);

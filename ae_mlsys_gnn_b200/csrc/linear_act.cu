@@ -1,0 +1,308 @@
+// Entry points of the linear layer with bias, activation and residual, and the elementwise half of
+// its gradient.
+//
+//   forward        z = x W^T + b,  y = act(z) + residual
+//   elementwise    gz = grad_y * act'(z),  grad_b = sum_rows gz
+//   products       grad_x = gz W,  grad_W = gz^T x
+//
+// 16-bit and 8-bit products run on linear_tc.cu, fp32 ones on the error-compensated 3xTF32 kernel
+// with the same epilogue.  The tensor cores truncate when they add (about 2^-26 of the value per
+// step), so the fp32 kernel moves its sums to registers after every kChain32 blocks of 32: 48 steps
+// stay below one unit in the last place of fp32.
+#include <stdio.h>
+#include <type_traits>
+#include "activation.cuh"
+#include "common.cuh"
+#include "dtypes.cuh"
+#include "gemm_persistent.cuh"
+#include "linear_tc.cuh"
+
+namespace gnn {
+namespace {
+
+constexpr int kChain32 = 2;
+constexpr int kGroupCols = 8;  // columns a thread owns in the elementwise gradient
+
+int fail(int code, const char* what, const char* why) {
+  char msg[256];
+  snprintf(msg, sizeof msg, "%s: %s", what, why);
+  set_last_error(msg);
+  return code;
+}
+
+struct ActBwdParams {
+  const void* gy;
+  const void* z;    // nullptr: no activation
+  void* gz;         // nullptr: not wanted
+  float* partial;   // [gridDim.y][N] column sums, nullptr: not wanted
+  int64_t M, rows_per_cta;
+  int N, ldz, groups;  // ldz: elements from one row of gz to the next; groups: threads across columns (2^k <= 32)
+  int act;
+  float slope;
+  int vec_ok;
+};
+
+// A CTA walks `rows_per_cta` rows of groups * 8 columns; a thread keeps its columns' sums in
+// registers.  HBM-bound: grad_y and z read, gz written once.
+template <class T>
+__global__ void __launch_bounds__(256) act_bwd_kernel(const ActBwdParams p) {
+  __shared__ float s_sum[256][kGroupCols + 1];
+  constexpr int V = 16 / (int)sizeof(T);
+  const int g = threadIdx.x & (p.groups - 1), strand = threadIdx.x / p.groups, strands = blockDim.x / p.groups;
+  const int col = (blockIdx.x * p.groups + g) * kGroupCols;
+  float sum[kGroupCols];
+#pragma unroll
+  for (int j = 0; j < kGroupCols; ++j) sum[j] = 0.f;
+  const int64_t lo = blockIdx.y * p.rows_per_cta, hi = min(lo + p.rows_per_cta, p.M);
+  const T* const gy = static_cast<const T*>(p.gy);
+  const T* const z = static_cast<const T*>(p.z);
+  T* const gz = static_cast<T*>(p.gz);
+  if (col < p.ldz) {
+#pragma unroll 2
+    for (int64_t row = lo + strand; row < hi; row += strands) {
+      const int64_t at = row * p.N + col;
+      float v[kGroupCols], a[kGroupCols];
+      if (p.vec_ok) {
+#pragma unroll
+        for (int i = 0; i < kGroupCols; i += V) {
+          const Pack<T, V> q = load_pack(reinterpret_cast<const Pack<T, V>*>(gy + at + i));
+          Pack<T, V> r;
+          if (z) r = load_pack(reinterpret_cast<const Pack<T, V>*>(z + at + i));
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            v[i + j] = to_f32(q.v[j]);
+            if (z) a[i + j] = to_f32(r.v[j]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kGroupCols; ++j) {
+          const bool ok = col + j < p.N;
+          v[j] = ok ? to_f32(gy[at + j]) : 0.f;
+          a[j] = ok && z ? to_f32(z[at + j]) : 0.f;
+        }
+      }
+      if (z) apply_act_slope<sizeof(T) == 4>(v, a, p.act, p.slope);
+#pragma unroll
+      for (int j = 0; j < kGroupCols; ++j) sum[j] += v[j];
+      if (gz) {
+        T* const o = gz + row * p.ldz + col;
+        if (p.vec_ok) {
+#pragma unroll
+          for (int i = 0; i < kGroupCols; i += V) {
+            Pack<T, V> q;
+#pragma unroll
+            for (int j = 0; j < V; ++j) q.v[j] = from_f32<T>(v[i + j]);
+            store_pack(reinterpret_cast<Pack<T, V>*>(o + i), q);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < kGroupCols; ++j)
+            if (col + j < p.ldz) o[j] = from_f32<T>(v[j]);  // the columns behind N are zeros
+        }
+      }
+    }
+  }
+  if (!p.partial) return;
+#pragma unroll
+  for (int j = 0; j < kGroupCols; ++j) s_sum[threadIdx.x][j] = sum[j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.groups * kGroupCols; i += blockDim.x) {
+    const int c = blockIdx.x * p.groups * kGroupCols + i;
+    if (c < p.N) {
+      float s = 0.f;
+      for (int r = 0; r < strands; ++r) s += s_sum[r * p.groups + i / kGroupCols][i % kGroupCols];
+      p.partial[(size_t)blockIdx.y * p.N + c] = s;
+    }
+  }
+}
+
+// out[col] = sum of the CTAs' column sums, in a fixed order.
+template <class W>
+__global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restrict__ partial, int parts, int n, W* out) {
+  __shared__ float s[32][33];
+  const int col = blockIdx.x * 32 + threadIdx.x;
+  float v = 0.f;
+  if (col < n)
+    for (int r = threadIdx.y; r < parts; r += 32) v += partial[(size_t)r * n + col];
+  s[threadIdx.y][threadIdx.x] = v;
+  __syncthreads();
+  v = warp_sum(s[threadIdx.x][threadIdx.y]);
+  const int c = blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x == 0 && c < n) out[c] = from_f32<W>(v);
+}
+
+struct ActBwdGrid {
+  int groups, col_ctas, row_ctas;
+  int64_t rows_per_cta;
+};
+ActBwdGrid act_bwd_grid(int64_t M, int64_t ldz) {
+  ActBwdGrid g;
+  const int64_t need = (ldz + kGroupCols - 1) / kGroupCols;
+  g.groups = 1;
+  while (g.groups < 32 && g.groups < need) g.groups *= 2;
+  g.col_ctas = (int)((need + g.groups - 1) / g.groups);
+  const int strands = 256 / g.groups;
+  int64_t rows = (148 * 8 + g.col_ctas - 1) / g.col_ctas;  // about eight CTAs an SM
+  const int64_t most = (M + 2 * strands - 1) / (2 * strands);
+  if (rows > most) rows = most;
+  if (rows < 1) rows = 1;
+  g.rows_per_cta = (M + rows - 1) / rows;
+  g.row_ctas = (int)((M + g.rows_per_cta - 1) / g.rows_per_cta);
+  return g;
+}
+
+int check_sizes(const char* what, int64_t M, int64_t N, int64_t K) {
+  if (M < 0 || N < 1 || K < 1) return fail(GNN_ERR_INVALID_ARG, what, "bad size");
+  if (M >= (1LL << 31) || N >= (1LL << 31) || K >= (1LL << 31)) return fail(GNN_ERR_LIMIT, what, "size exceeds int32");
+  return GNN_OK;
+}
+
+bool is_float(int t) { return dtype_bytes(t) != 0; }
+
+}  // namespace
+}  // namespace gnn
+
+using namespace gnn;
+
+extern "C" int gnn_linear_fwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int in_type, size_t* bytes) {
+  if (!bytes || M < 0 || N < 1 || K < 1 || in_type < GNN_F32 || in_type > GNN_E4M3)
+    return fail(GNN_ERR_INVALID_ARG, "gnn_linear_fwd_workspace_bytes", "bad argument");
+  if (in_type == GNN_F32) return gnn_gemm_tf32x3_workspace_bytes(M, N, K, bytes);
+  *bytes = linear_tc_workspace(M, N, K, in_type);
+  return GNN_OK;
+}
+
+extern "C" int gnn_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int in_type, const float* x_scale,
+                              const float* w_scale, const void* bias, int act, float slope, const void* residual, void* y,
+                              void* z, int out_type, int64_t M, int64_t N, int64_t K, void* workspace,
+                              size_t workspace_bytes, int* status, cudaStream_t stream) {
+  const char* const what = "gnn_linear_fwd";
+  if (int rc = check_sizes(what, M, N, K)) return rc;
+  if (in_type < GNN_F32 || in_type > GNN_E4M3 || !is_float(out_type) || (in_type != GNN_E4M3 && in_type != out_type))
+    return fail(GNN_ERR_UNSUPPORTED, what, "operands are fp32, bf16, fp16 (and so is the output) or e4m3");
+  if (act < GNN_ACT_NONE || act > GNN_ACT_SILU) return fail(GNN_ERR_INVALID_ARG, what, "unknown activation");
+  if ((in_type == GNN_E4M3) != (x_scale != nullptr) || (in_type == GNN_E4M3) != (w_scale != nullptr))
+    return fail(GNN_ERR_INVALID_ARG, what, "e4m3 operands, and only they, come with their scales");
+  if (M == 0) return GNN_OK;
+  if (!x || !w || !y || !status) return fail(GNN_ERR_INVALID_ARG, what, "null pointer");
+  if (ldx < K || ldw < K) return fail(GNN_ERR_INVALID_ARG, what, "a row is shorter than K");
+  if (in_type == GNN_F32) {
+    if (ldx != K || ldw != K) return fail(GNN_ERR_UNSUPPORTED, what, "fp32 rows must be K elements apart");
+    const GemmFinish fin{static_cast<const float*>(bias), static_cast<float*>(z), act, slope,
+                         static_cast<const float*>(residual)};
+    return tf32x3_product(static_cast<const float*>(x), static_cast<const float*>(w), 1, static_cast<float*>(y), M, N, K,
+                          workspace, workspace_bytes, status, stream, nullptr, &fin, kChain32, what);
+  }
+  const TcOperand a{x, ldx, false}, b{w, ldw, false};
+  const int elt = in_type == GNN_E4M3 ? 1 : 2;
+  if (!tma_operand_ok(a, elt) || !tma_operand_ok(b, elt))
+    return fail(GNN_ERR_UNSUPPORTED, what, "rows must start on 16-byte boundaries");
+  const LinearEpilogue ep{x_scale, w_scale, bias, z, act, slope, residual, y, out_type};
+  return launch_linear_tc(a, b, in_type, M, N, K, ep, workspace, workspace_bytes, status, stream, what);
+}
+
+extern "C" int gnn_linear_act_bwd_workspace_bytes(int64_t M, int64_t N, int64_t ldz, size_t* bytes) {
+  if (!bytes || M < 0 || N < 1 || ldz < N)
+    return fail(GNN_ERR_INVALID_ARG, "gnn_linear_act_bwd_workspace_bytes", "bad argument");
+  *bytes = (size_t)(M ? act_bwd_grid(M, ldz).row_ctas : 1) * N * sizeof(float) + 16;
+  return GNN_OK;
+}
+
+extern "C" int gnn_linear_act_bwd(const void* grad_y, const void* z, int act, float slope, int dtype, int64_t M, int64_t N,
+                                  void* gz, int64_t ldz, void* grad_b, void* workspace, size_t workspace_bytes,
+                                  cudaStream_t stream) {
+  const char* const what = "gnn_linear_act_bwd";
+  if (int rc = check_sizes(what, M, N, 1)) return rc;
+  if (!is_float(dtype)) return fail(GNN_ERR_UNSUPPORTED, what, "rows are fp32, bf16 or fp16");
+  if (act < GNN_ACT_NONE || act > GNN_ACT_SILU) return fail(GNN_ERR_INVALID_ARG, what, "unknown activation");
+  if (ldz < N || ldz >= (1LL << 31)) return fail(GNN_ERR_INVALID_ARG, what, "bad row length of gz");
+  if (M == 0) {
+    if (grad_b) cudaMemsetAsync(grad_b, 0, (size_t)N * dtype_bytes(dtype), stream);
+    return check_launch(what);
+  }
+  if (!grad_y || (act && !z) || (!gz && !grad_b)) return fail(GNN_ERR_INVALID_ARG, what, "null pointer");
+  size_t need = 0;
+  gnn_linear_act_bwd_workspace_bytes(M, N, ldz, &need);
+  if (grad_b && (!workspace || workspace_bytes < need)) return fail(GNN_ERR_WORKSPACE, what, "workspace too small");
+  const ActBwdGrid g = act_bwd_grid(M, ldz);
+  float* const partial = grad_b ? (float*)(((uintptr_t)workspace + 15) & ~(uintptr_t)15) : nullptr;
+  const uintptr_t all = (uintptr_t)grad_y | (act ? (uintptr_t)z : 0) | (uintptr_t)gz;
+  ActBwdParams p{grad_y, act ? z : nullptr, gz, partial, M, g.rows_per_cta, (int)N, (int)ldz, g.groups, act, slope,
+                 N % 8 == 0 && ldz == N && all % 16 == 0};
+  const dim3 grid((unsigned)g.col_ctas, (unsigned)g.row_ctas);
+  if (g.row_ctas > 65535) return fail(GNN_ERR_LIMIT, what, "too many rows");
+  if (dtype == GNN_F32) act_bwd_kernel<float><<<grid, 256, 0, stream>>>(p);
+  else if (dtype == GNN_BF16) act_bwd_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(p);
+  else act_bwd_kernel<__half><<<grid, 256, 0, stream>>>(p);
+  if (grad_b) {
+    const unsigned cols = (unsigned)((N + 31) / 32);
+    const dim3 block(32, 32);
+    if (dtype == GNN_F32) column_sum_kernel<<<cols, block, 0, stream>>>(partial, g.row_ctas, (int)N, (float*)grad_b);
+    else if (dtype == GNN_BF16) column_sum_kernel<<<cols, block, 0, stream>>>(partial, g.row_ctas, (int)N, (__nv_bfloat16*)grad_b);
+    else column_sum_kernel<<<cols, block, 0, stream>>>(partial, g.row_ctas, (int)N, (__half*)grad_b);
+  }
+  return check_launch(what);
+}
+
+extern "C" int gnn_linear_dgrad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, size_t* bytes) {
+  if (!bytes || M < 0 || N < 1 || K < 1 || !is_float(dtype))
+    return fail(GNN_ERR_INVALID_ARG, "gnn_linear_dgrad_workspace_bytes", "bad argument");
+  if (dtype == GNN_F32) return gnn_gemm_tf32x3_workspace_bytes(M, K, N, bytes);
+  *bytes = linear_tc_workspace(M, K, N, dtype);
+  return GNN_OK;
+}
+
+extern "C" int gnn_linear_dgrad(const void* gz, int64_t ldg, const void* w, int64_t ldw, int dtype, void* grad_x, int64_t M,
+                                int64_t N, int64_t K, void* workspace, size_t workspace_bytes, int* status,
+                                cudaStream_t stream) {
+  const char* const what = "gnn_linear_dgrad";
+  if (int rc = check_sizes(what, M, N, K)) return rc;
+  if (!is_float(dtype)) return fail(GNN_ERR_UNSUPPORTED, what, "operands are fp32, bf16 or fp16");
+  if (M == 0) return GNN_OK;
+  if (!gz || !w || !grad_x || !status) return fail(GNN_ERR_INVALID_ARG, what, "null pointer");
+  if (ldg < N || ldw < K) return fail(GNN_ERR_INVALID_ARG, what, "a row is shorter than its columns");
+  if (dtype == GNN_F32) {
+    if (ldg != N || ldw != K) return fail(GNN_ERR_UNSUPPORTED, what, "fp32 rows must lie one after the other");
+    const GemmFinish plain{};
+    return tf32x3_product(static_cast<const float*>(gz), static_cast<const float*>(w), 0, static_cast<float*>(grad_x), M, K,
+                          N, workspace, workspace_bytes, status, stream, nullptr, &plain, kChain32, what);
+  }
+  const TcOperand a{gz, ldg, false}, b{w, ldw, true};
+  if (!tma_operand_ok(a, 2) || !tma_operand_ok(b, 2))
+    return fail(GNN_ERR_UNSUPPORTED, what, "rows must start on 16-byte boundaries");
+  const LinearEpilogue ep{nullptr, nullptr, nullptr, nullptr, GNN_ACT_NONE, 0.f, nullptr, grad_x, dtype};
+  return launch_linear_tc(a, b, dtype, M, K, N, ep, workspace, workspace_bytes, status, stream, what);
+}
+
+extern "C" int gnn_linear_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, size_t* bytes) {
+  if (!bytes || M < 0 || N < 1 || K < 1 || !is_float(dtype))
+    return fail(GNN_ERR_INVALID_ARG, "gnn_linear_wgrad_workspace_bytes", "bad argument");
+  if (dtype == GNN_F32) return gnn_gemm_tf32x3_tn_workspace_bytes(M, N, K, bytes);
+  *bytes = linear_tc_workspace(N, K, M, dtype);
+  return GNN_OK;
+}
+
+extern "C" int gnn_linear_wgrad(const void* gz, int64_t ldg, const void* x, int64_t ldx, int dtype, void* grad_w, int64_t M,
+                                int64_t N, int64_t K, void* workspace, size_t workspace_bytes, int* status,
+                                cudaStream_t stream) {
+  const char* const what = "gnn_linear_wgrad";
+  if (int rc = check_sizes(what, M, N, K)) return rc;
+  if (!is_float(dtype)) return fail(GNN_ERR_UNSUPPORTED, what, "operands are fp32, bf16 or fp16");
+  if (!grad_w || !status || (M && (!gz || !x))) return fail(GNN_ERR_INVALID_ARG, what, "null pointer");
+  if (M == 0) {
+    cudaMemsetAsync(grad_w, 0, (size_t)N * K * dtype_bytes(dtype), stream);
+    return check_launch(what);
+  }
+  if (ldg < N || ldx < K) return fail(GNN_ERR_INVALID_ARG, what, "a row is shorter than its columns");
+  if (dtype == GNN_F32) {
+    if (ldg != N || ldx != K) return fail(GNN_ERR_UNSUPPORTED, what, "fp32 rows must lie one after the other");
+    return tf32x3_product_tn(static_cast<const float*>(gz), static_cast<const float*>(x), static_cast<float*>(grad_w), M, N,
+                             K, workspace, workspace_bytes, status, stream, kChain32);
+  }
+  const TcOperand a{gz, ldg, true}, b{x, ldx, true};
+  if (!tma_operand_ok(a, 2) || !tma_operand_ok(b, 2))
+    return fail(GNN_ERR_UNSUPPORTED, what, "rows must start on 16-byte boundaries");
+  const LinearEpilogue ep{nullptr, nullptr, nullptr, nullptr, GNN_ACT_NONE, 0.f, nullptr, grad_w, dtype};
+  return launch_linear_tc(a, b, dtype, N, K, M, ep, workspace, workspace_bytes, status, stream, what);
+}

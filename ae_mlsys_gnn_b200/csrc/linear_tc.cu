@@ -1,0 +1,718 @@
+// Product of 16-bit or 8-bit operands on the 5th-generation tensor cores with a fused epilogue:
+//
+//   out[m,n] = act(row_scale[m] * col_scale[n] * sum_k A[m,k] * B[n,k] + bias[n]) + residual[m,n]
+//
+// fp32 accumulation in tensor memory, fp32 epilogue, one rounding.  Persistent and warp-specialised:
+//   warp 0      TMA producer: a stage is 128 bytes along the reduction axis of both operands
+//   warp 1      tensor-memory allocation and single-thread tcgen05.mma issue
+//   warps 2-9   epilogue: two warps per 32 rows, alternate 32-column chunks
+// The accumulator is double buffered in tensor memory, so the epilogue of a tile runs under the main
+// loop of the next one.
+//
+// kPair: two CTAs of a cluster (the two SMs of a TPC) work on one 256 x 256 tile with
+// cta_group::2 MMAs.  Each holds its own 128 rows of A and half of B in shared memory, so a
+// multiply-add reads 2/3 of the shared-memory bytes that a 128 x 128 tile of one CTA reads per operand
+// row, and only half of B is fetched per CTA.  The even CTA issues the MMAs for both.
+//
+// Operands whose reduction axis is the slow one in memory (the weights in the input's gradient, both
+// operands in the weights' gradient) are loaded as MN-major tiles: boxes of 64 columns x 64
+// reduction rows, no transposed copies.
+//
+// Every mbarrier wait is bounded in time: on expiry the CTA raises a flag that ends all its loops,
+// sets the status word, gives its copies in flight a bounded time to land, frees its tensor memory
+// and returns.
+#include <cuda.h>
+#include <stdio.h>
+#include "activation.cuh"
+#include "common.cuh"
+#include "dtypes.cuh"
+#include "linear_tc.cuh"
+
+namespace gnn {
+namespace {
+
+constexpr int BM = 128;             // rows per CTA
+constexpr int kStageK = 128;        // bytes of a stage along the reduction axis
+constexpr int kATile = BM * kStageK;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 32 * (2 + kEpiWarps);
+constexpr int kMaxStages = 7;
+constexpr int kNumBars = 2 * kMaxStages + 4;
+constexpr int kBarBytes = (8 * kNumBars + 16 + 127) / 128 * 128;
+constexpr int kEpiBytes = kEpiWarps * 32 * 32 * 4;  // a 32 x 32 fp32 block per epilogue warp
+constexpr long long kWaitCycles = 4000000000LL;     // about two seconds
+constexpr long long kDrainCycles = 200000000LL;     // about a tenth of a second
+
+template <int BN, bool PAIR>
+struct Geom {
+  static constexpr int kBRows = PAIR ? BN / 2 : BN;  // B rows in this CTA's shared memory
+  static constexpr int kStageBytes = kATile + kBRows * kStageK;
+  static constexpr int kFit = (232448 - 1024 - kBarBytes - kEpiBytes) / kStageBytes;
+  static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
+  static constexpr int kTmemCols = 2 * BN;
+  static constexpr size_t kSmemBytes = (size_t)kStages * kStageBytes + 1024 + kBarBytes + kEpiBytes;
+};
+
+struct Params {
+  int M, N;
+  int total_kb, kb_per_split;       // stages along the reduction axis
+  int tiles_m, tiles_n, num_tiles;  // num_tiles = tiles_m * tiles_n * splits
+  int a_mn, b_mn;
+  int k_elems;                      // elements of a stage along the reduction axis
+  uint32_t idesc;                   // instruction descriptor without the N field
+  float* planes;                    // splits > 1: fp32 partial planes [splits][M][N]
+  int vec_ok;                       // whole 16-byte accesses of out, z, residual and bias
+  LinearEpilogue ep;
+  int* status;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Arrives at the barrier of the same offset in the cluster's CTA `rank`.
+__device__ __forceinline__ void mbar_arrive_at(uint32_t bar, uint32_t rank) {
+  asm volatile(
+      "{\n\t.reg .b32 r;\n\t"
+      "mapa.shared::cluster.u32 r, %0, %1;\n\t"
+      "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n\t}" ::"r"(bar), "r"(rank) : "memory");
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* failed,
+                                          long long limit = kWaitCycles) {
+  const long long t0 = clock64();
+  for (uint32_t i = 0;; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (ok) return true;
+    if ((i & 15) == 15) {
+      if (failed && *failed) return false;
+      if (clock64() - t0 > limit) return false;
+    }
+  }
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");
+}
+
+// A pair's copies report to the even CTA's barrier: the same offset with the CTA bit cleared.
+template <bool PAIR>
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  if constexpr (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(bar & 0xFEFFFFFFu) : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(bar) : "memory");
+}
+
+// Shared-memory matrix descriptors (version 1, 128-byte swizzle).
+//   K-major tile [rows][128 bytes]: 8-row groups 1024 bytes apart (stride offset), the leading
+//   offset is not used; a K slice of one MMA is 32 bytes further.
+//   MN-major tile [groups of 64 columns][64 reduction rows][128 bytes] of 16-bit elements: column
+//   groups 8192 bytes apart (leading offset), 8 reduction rows 1024 bytes apart (stride offset); a
+//   K slice of 16 is 2048 bytes further.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t saddr, bool mn_major) {
+  uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFF);
+  d |= (uint64_t)((mn_major ? 8192 : 16) >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+template <bool PAIR, bool FP8>
+__device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+#define GNN_UMMA(GROUP, KIND)                                              \
+  asm volatile(                                                            \
+      "{\n\t.reg .pred p;\n\t"                                             \
+      "setp.ne.b32 p, %4, 0;\n\t"                                          \
+      "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, p;\n\t}" \
+      ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate) : "memory")
+  if constexpr (PAIR) {
+    if constexpr (FP8) GNN_UMMA("2", "f8f6f4");
+    else GNN_UMMA("2", "f16");
+  } else {
+    if constexpr (FP8) GNN_UMMA("1", "f8f6f4");
+    else GNN_UMMA("1", "f16");
+  }
+#undef GNN_UMMA
+}
+// Arrives at the barrier (of both CTAs of a pair) once the MMAs issued so far are done.
+template <bool PAIR>
+__device__ __forceinline__ void umma_commit(uint32_t bar) {
+  if constexpr (PAIR)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+        ::"r"(bar), "h"((uint16_t)3) : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+struct TileCoord {
+  int m0, n0, kb_begin, num_kb, z;
+};
+// Tiles in bands of 8 row tiles, column by column inside a band: the CTAs that run at the same time
+// share rows of A and of B through L2.
+template <int TM, int TN>
+__device__ __forceinline__ TileCoord decode_tile(const Params& p, int tile) {
+  constexpr int kBand = 8;
+  const int per_split = p.tiles_m * p.tiles_n;
+  TileCoord t;
+  t.z = tile / per_split;
+  const int i = tile - t.z * per_split;
+  const int band = i / (kBand * p.tiles_n);
+  const int high = min(kBand, p.tiles_m - band * kBand);
+  const int j = i - band * kBand * p.tiles_n;
+  const int nt = j / high;
+  t.m0 = (band * kBand + j - nt * high) * TM;
+  t.n0 = nt * TN;
+  t.kb_begin = t.z * p.kb_per_split;
+  t.num_kb = max(0, min(p.kb_per_split, p.total_kb - t.kb_begin));
+  return t;
+}
+
+// Eight consecutive values of type T at p (16-byte aligned), widened.
+template <class T>
+__device__ __forceinline__ void load8(const T* p, float (&o)[8]) {
+  constexpr int V = 16 / (int)sizeof(T);
+#pragma unroll
+  for (int i = 0; i < 8; i += V) {
+    const Pack<T, V> a = load_pack(reinterpret_cast<const Pack<T, V>*>(p + i));
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[i + j] = to_f32(a.v[j]);
+  }
+}
+template <class T>
+__device__ __forceinline__ void store8(T* p, const float (&o)[8]) {
+  constexpr int V = 16 / (int)sizeof(T);
+#pragma unroll
+  for (int i = 0; i < 8; i += V) {
+    Pack<T, V> a;
+#pragma unroll
+    for (int j = 0; j < V; ++j) a.v[j] = from_f32<T>(o[i + j]);
+    store_pack(reinterpret_cast<Pack<T, V>*>(p + i), a);
+  }
+}
+
+// The epilogue of one element, for outputs whose rows are not whole 16-byte units.
+template <class T>
+__device__ __forceinline__ void finish_one(const LinearEpilogue& ep, int64_t row, int col, int N, float v) {
+  const int64_t at = row * N + col;
+  if (ep.col_scale) v *= __ldg(ep.row_scale + row) * __ldg(ep.col_scale + col);
+  if (ep.bias) v += to_f32(static_cast<const T*>(ep.bias)[col]);
+  if (ep.z) static_cast<T*>(ep.z)[at] = from_f32<T>(v);
+  v = act_value<sizeof(T) == 4>(v, ep.act, ep.slope);
+  if (ep.residual) v += to_f32(static_cast<const T*>(ep.residual)[at]);
+  static_cast<T*>(ep.out)[at] = from_f32<T>(v);
+}
+
+// Eight columns of kRows rows at a time: residual, bias and scales are requested early, and the
+// activation is one branch for all 8 * kRows values.
+template <class T, int kRows>
+struct Finish8 {
+  static constexpr int V = 16 / (int)sizeof(T), Q = 8 / V;
+  Pack<T, V> residual[kRows][Q];
+  float bias[8], scale[8], row_scale[kRows];
+
+  // rows row0 + step * i; in(i): the row exists
+  template <class In>
+  __device__ __forceinline__ void request(const LinearEpilogue& ep, int64_t row0, int step, int col, int N, In&& in) {
+    if (ep.residual) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i)
+        if (in(i)) {
+          const T* const at = static_cast<const T*>(ep.residual) + (row0 + step * i) * N + col;
+#pragma unroll
+          for (int q = 0; q < Q; ++q) residual[i][q] = load_pack(reinterpret_cast<const Pack<T, V>*>(at) + q);
+        }
+    }
+  }
+  template <class In>
+  __device__ __forceinline__ void columns(const LinearEpilogue& ep, int64_t row0, int step, int col, bool ok, In&& in) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bias[j] = 0.f;
+    if (ep.bias && ok) load8(static_cast<const T*>(ep.bias) + col, bias);
+    if (ep.col_scale) {
+      if (ok) load8(ep.col_scale + col, scale);
+#pragma unroll
+      for (int i = 0; i < kRows; ++i)
+        if (in(i)) row_scale[i] = __ldg(ep.row_scale + row0 + step * i);
+    }
+  }
+  template <class In>
+  __device__ __forceinline__ void finish(const LinearEpilogue& ep, int64_t row0, int step, int col, int N, In&& in,
+                                         float (&v)[kRows * 8]) {
+    if (ep.col_scale) {
+#pragma unroll
+      for (int i = 0; i < kRows * 8; ++i) v[i] *= row_scale[i / 8] * scale[i % 8];
+    }
+#pragma unroll
+    for (int i = 0; i < kRows * 8; ++i) v[i] += bias[i % 8];
+    if (ep.z) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i)
+        if (in(i)) store_row(static_cast<T*>(ep.z) + (row0 + step * i) * N + col, v, i);
+    }
+    apply_act<sizeof(T) == 4>(v, ep.act, ep.slope);
+    if (ep.residual) {
+#pragma unroll
+      for (int i = 0; i < kRows * 8; ++i) v[i] += to_f32(residual[i / 8][i % 8 / V].v[i % V]);
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+      if (in(i)) store_row(static_cast<T*>(ep.out) + (row0 + step * i) * N + col, v, i);
+  }
+  __device__ __forceinline__ static void store_row(T* at, const float (&v)[kRows * 8], int i) {
+    float o[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = v[i * 8 + j];
+    store8(at, o);
+  }
+};
+
+template <int BN, bool PAIR, bool FP8, class T>
+__global__ void __launch_bounds__(kThreads, 1)
+linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
+  using G = Geom<BN, PAIR>;
+  constexpr int kStages = G::kStages;
+  constexpr int TM = PAIR ? 2 * BM : BM;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t base = (raw_addr + 1023u) & ~1023u;  // swizzle atoms need 1024-byte alignment
+  uint8_t* const base_ptr = smem_raw + (base - raw_addr);
+  const uint32_t bars = base + kStages * G::kStageBytes;
+  auto full_bar = [&](int s) { return bars + 8u * s; };                             // TMA -> MMA
+  auto empty_bar = [&](int s) { return bars + 8u * (kMaxStages + s); };             // MMA -> TMA
+  auto acc_full_bar = [&](int b) { return bars + 8u * (2 * kMaxStages + b); };      // MMA -> epilogue
+  auto acc_empty_bar = [&](int b) { return bars + 8u * (2 * kMaxStages + 2 + b); }; // epilogue -> MMA
+  const uint32_t tmem_slot = bars + 8u * kNumBars;
+  float4* const epi = reinterpret_cast<float4*>(base_ptr + kStages * G::kStageBytes + kBarBytes);
+
+  __shared__ volatile int s_failed;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_rank() : 0;
+  const int unit = PAIR ? blockIdx.x >> 1 : blockIdx.x, units = PAIR ? gridDim.x >> 1 : gridDim.x;
+
+  if (threadIdx.x == 0) {
+    s_failed = 0;
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full_bar(b), 1);
+      mbar_init(acc_empty_bar(b), kEpiWarps * (PAIR ? 2 : 1));
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(G::kTmemCols) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(G::kTmemCols) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // the other CTA's barriers exist
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(base_ptr + kStages * G::kStageBytes + 8 * kNumBars);
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- TMA producer
+    if (lane == 0) {
+      uint32_t it = 0;
+      for (int tile = unit; tile < p.num_tiles && !s_failed; tile += units) {
+        const TileCoord t = decode_tile<TM, BN>(p, tile);
+        const int a_row = t.m0 + (int)rank * BM, b_row = t.n0 + (int)rank * G::kBRows;
+        for (int kb = 0; kb < t.num_kb; ++kb, ++it) {
+          const int s = it % kStages;
+          const uint32_t round = it / kStages;
+          if (round > 0 && !mbar_wait(empty_bar(s), (round - 1) & 1, &s_failed)) { s_failed = 1; break; }
+          const uint32_t st = base + s * G::kStageBytes;
+          const int k0 = (t.kb_begin + kb) * p.k_elems;
+          if (rank == 0) mbar_expect_tx(full_bar(s), G::kStageBytes * (PAIR ? 2 : 1));
+          if (p.a_mn) {
+#pragma unroll
+            for (int g = 0; g < BM / 64; ++g) tma_load<PAIR>(st + g * 8192, &map_a, a_row + 64 * g, k0, full_bar(s));
+          } else {
+            tma_load<PAIR>(st, &map_a, k0, a_row, full_bar(s));
+          }
+          if (p.b_mn) {
+#pragma unroll
+            for (int g = 0; g < G::kBRows / 64; ++g)
+              tma_load<PAIR>(st + kATile + g * 8192, &map_b, b_row + 64 * g, k0, full_bar(s));
+          } else {
+            tma_load<PAIR>(st + kATile, &map_b, k0, b_row, full_bar(s));
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issue
+    if (lane == 0 && rank == 0) {
+      const uint64_t a_step = p.a_mn ? (2048 >> 4) : (32 >> 4);  // descriptor advance per K slice
+      const uint64_t b_step = p.b_mn ? (2048 >> 4) : (32 >> 4);
+      const uint32_t idesc = p.idesc | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
+      uint32_t it = 0, count = 0;
+      bool ok = true;
+      for (int tile = unit; tile < p.num_tiles && ok && !s_failed; tile += units, ++count) {
+        const TileCoord t = decode_tile<TM, BN>(p, tile);
+        const int buf = count & 1;
+        // a fresh barrier lets the wait for parity 1 through: the first use of a buffer does not block
+        if (!mbar_wait(acc_empty_bar(buf), ((count >> 1) & 1) ^ 1, &s_failed)) { s_failed = 1; break; }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t acc = tmem_base + (uint32_t)(buf * BN);
+        for (int kb = 0; kb < t.num_kb; ++kb, ++it) {
+          const int s = it % kStages;
+          if (!mbar_wait(full_bar(s), (it / kStages) & 1, &s_failed)) { s_failed = 1; ok = false; break; }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t st = base + s * G::kStageBytes;
+          const uint64_t da = operand_desc(st, p.a_mn), db = operand_desc(st + kATile, p.b_mn);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma<PAIR, FP8>(acc, da + a_step * k, db + b_step * k, idesc, (kb | k) != 0);
+          umma_commit<PAIR>(empty_bar(s));  // the stage is free once these MMAs have read it
+        }
+        if (ok) umma_commit<PAIR>(acc_full_bar(buf));
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- epilogue
+    const int lg = warp & 3;            // this warp may touch tensor-memory lanes [32*lg, 32*lg + 32)
+    const int half = (warp - 2) >> 2;   // even or odd 32-column chunks
+    float4* const stg = epi + (warp - 2) * 256;
+    const int sub = lane >> 2, oct = lane & 3;  // row of 8 and 8-column group this lane finishes
+    uint32_t count = 0;
+    for (int tile = unit; tile < p.num_tiles && !s_failed; tile += units, ++count) {
+      const TileCoord t = decode_tile<TM, BN>(p, tile);
+      const int buf = count & 1;
+      const int64_t row0 = t.m0 + (int)rank * BM + lg * 32 + sub;  // this lane's rows: row0 + 8 i
+      Finish8<T, 4> fin;
+      const bool whole = p.vec_ok && !p.planes;
+      auto in = [&](int col) { return [=](int i) { return row0 + 8 * i < p.M && col < p.N; }; };
+      if (whole) {  // the first chunk's residual is under way while the product finishes
+        const int col = t.n0 + half * 32 + oct * 8;
+        fin.request(p.ep, row0, 8, col, p.N, in(col));
+      }
+      if (!mbar_wait(acc_full_bar(buf), (count >> 1) & 1, &s_failed)) { s_failed = 1; break; }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+      for (int c = half; c < BN / 32; c += 2) {
+        const int col0 = t.n0 + c * 32;
+        if (col0 >= p.N) break;
+        uint32_t r[32];
+        const uint32_t taddr = tmem_base + ((uint32_t)(lg * 32) << 16) + (uint32_t)(buf * BN + c * 32);
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+            "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+            "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+              "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+              "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+              "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+            : "r"(taddr) : "memory");
+        const int col = col0 + oct * 8;
+        if (whole) fin.columns(p.ep, row0, 8, col, col < p.N, in(col));
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (t.num_kb == 0) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[j] = 0u;  // an empty range contributes nothing
+        }
+        // Through shared memory from one row per lane to four lanes per row, so that a warp
+        // instruction covers 64-byte pieces of 8 rows; the 16-byte units of row r are rotated by
+        // r mod 8, which keeps both sides free of bank conflicts.
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          stg[lane * 8 + (j ^ (lane & 7))] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
+                                                         __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
+        __syncwarp();
+        if (p.vec_ok) {
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int rr = i * 8 + sub;
+            const float4 lo = stg[rr * 8 + ((oct * 2) ^ (rr & 7))], hi = stg[rr * 8 + ((oct * 2 + 1) ^ (rr & 7))];
+            v[8 * i] = lo.x; v[8 * i + 1] = lo.y; v[8 * i + 2] = lo.z; v[8 * i + 3] = lo.w;
+            v[8 * i + 4] = hi.x; v[8 * i + 5] = hi.y; v[8 * i + 6] = hi.z; v[8 * i + 7] = hi.w;
+          }
+          if (whole) {
+            fin.finish(p.ep, row0, 8, col, p.N, in(col), v);
+            if (c + 2 < BN / 32) fin.request(p.ep, row0, 8, col + 64, p.N, in(col + 64));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (in(col)(i)) Finish8<float, 4>::store_row(p.planes + ((size_t)t.z * p.M + row0 + 8 * i) * p.N + col, v, i);
+          }
+        } else {
+          // one element per lane and step: neighbours of a row on neighbouring lanes
+          const float* const flat = reinterpret_cast<const float*>(stg);
+          const int64_t top = t.m0 + (int)rank * BM + lg * 32;
+          if (col0 + lane < p.N) {
+#pragma unroll 1
+            for (int rr = 0; rr < 32 && top + rr < p.M; ++rr) {
+              const float v = flat[(rr * 8 + ((lane >> 2) ^ (rr & 7))) * 4 + (lane & 3)];
+              if (p.planes) p.planes[((size_t)t.z * p.M + top + rr) * p.N + col0 + lane] = v;
+              else finish_one<T>(p.ep, top + rr, col0 + lane, p.N, v);
+            }
+          }
+        }
+        __syncwarp();  // the block is rewritten by the next chunk
+      }
+      // the buffer may be overwritten once every epilogue warp has read it
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (PAIR) mbar_arrive_at(acc_empty_bar(buf), 0);
+        else mbar_arrive(acc_empty_bar(buf));
+      }
+    }
+  }
+
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (s_failed) {
+    // something expired: give the copies still in flight a bounded time to land before the shared
+    // memory is released
+    if (threadIdx.x == 0) {
+      *p.status = 1;
+      for (int s = 0; s < kStages; ++s) {
+        mbar_wait(full_bar(s), 0, nullptr, kDrainCycles);
+        mbar_wait(full_bar(s), 1, nullptr, kDrainCycles);
+      }
+    }
+    __syncthreads();
+  }
+  if constexpr (PAIR) cluster_sync();  // neither CTA leaves while the other may still signal it
+  if (warp == 1) {
+    __syncwarp();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if constexpr (PAIR)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(G::kTmemCols) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(G::kTmemCols) : "memory");
+  }
+}
+
+// Sums the fp32 planes of a split product in order and finishes the row pieces.
+template <class T>
+__global__ void __launch_bounds__(256) split_epilogue_kernel(const float* __restrict__ planes, int parts, int64_t M, int N, int octs,
+                                                             int vec_ok, const LinearEpilogue ep) {
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int64_t row = i / octs;
+  if (row >= M) return;
+  const int col = (int)(i - row * octs) * 8;
+  const size_t plane = (size_t)M * N;
+  const float* const at = planes + row * N + col;
+  if (vec_ok) {
+    Finish8<T, 1> fin;
+    auto in = [](int) { return true; };
+    fin.request(ep, row, 0, col, N, in);
+    fin.columns(ep, row, 0, col, true, in);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+#pragma unroll 4
+    for (int z = 0; z < parts; ++z) {
+      float f[8];
+      load8(at + z * plane, f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += f[j];
+    }
+    fin.finish(ep, row, 0, col, N, in, v);
+  } else {
+#pragma unroll 1
+    for (int j = 0; j < 8 && col + j < N; ++j) {
+      float v = 0.f;
+#pragma unroll 4
+      for (int z = 0; z < parts; ++z) v += at[z * plane + j];
+      finish_one<T>(ep, row, col + j, N, v);
+    }
+  }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+  static const EncodeTiledFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                   q == cudaDriverEntryPointSuccess
+               ? (EncodeTiledFn)p
+               : nullptr;
+  }();
+  return fn;
+}
+
+// Map over the stored matrix [outer][inner] with a box of 128 bytes x box_outer rows; zeros outside.
+bool encode(CUtensorMap* m, const TcOperand& o, int in_type, int64_t rows, int64_t K, int tile_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const int elt = in_type == GNN_E4M3 ? 1 : 2;
+  const CUtensorMapDataType dt = in_type == GNN_E4M3   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                 : in_type == GNN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  cuuint64_t dims[2] = {(cuuint64_t)(o.mn_major ? rows : K), (cuuint64_t)(o.mn_major ? K : rows)};
+  cuuint64_t strides[1] = {(cuuint64_t)o.ld * elt};
+  cuuint32_t box[2] = {(cuuint32_t)(128 / elt), (cuuint32_t)(o.mn_major ? 64 : tile_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(m, dt, 2, const_cast<void*>(o.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+         CUDA_SUCCESS;
+}
+
+struct Plan {
+  int bn, pair, splits;
+  int64_t tiles_m, tiles_n;
+};
+constexpr int kSms = 148;
+
+// Tile and split of the reduction axis for a shape.
+Plan plan_for(int64_t M, int64_t N, int64_t K, int in_type) {
+  const int64_t kb = (K * (in_type == GNN_E4M3 ? 1 : 2) + kStageK - 1) / kStageK;
+  Plan p;
+  auto tiles = [&](int tm, int tn) { return ((M + tm - 1) / tm) * ((N + tn - 1) / tn); };
+  p.pair = M > BM && tiles(256, 256) >= kSms / 2;
+  p.bn = p.pair ? 256 : (tiles(128, 128) >= kSms || N > 64 ? 128 : 64);
+  const int tm = p.pair ? 256 : 128;
+  p.tiles_m = (M + tm - 1) / tm;
+  p.tiles_n = (N + p.bn - 1) / p.bn;
+  const int64_t units = p.pair ? kSms / 2 : kSms, t = p.tiles_m * p.tiles_n;
+  int64_t s = units / t;              // fill the GPU
+  if (s > kb / 8) s = kb / 8;         // at least 8 stages a range
+  // the tensor cores add with truncation (about 2^-26 a step): no chain of more than 2048 stages
+  const int64_t least = (kb + 2047) / 2048;
+  if (s < least) s = least;
+  p.splits = s < 1 ? 1 : (int)s;
+  return p;
+}
+
+template <int BN, bool PAIR, bool FP8, class T>
+int launch_instance(const CUtensorMap& ma, const CUtensorMap& mb, const Params& p, int grid, cudaStream_t stream) {
+  using G = Geom<BN, PAIR>;
+  auto kernel = linear_tc_kernel<BN, PAIR, FP8, T>;
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)G::kSmemBytes);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = G::kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = PAIR ? 2 : 1;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, ma, mb, p) == cudaSuccess ? 0 : 1;
+}
+
+template <bool FP8, class T>
+int launch_shape(const Plan& pl, const CUtensorMap& ma, const CUtensorMap& mb, const Params& p, int grid, cudaStream_t stream) {
+  if (pl.pair) return launch_instance<256, true, FP8, T>(ma, mb, p, grid, stream);
+  if (pl.bn == 128) return launch_instance<128, false, FP8, T>(ma, mb, p, grid, stream);
+  return launch_instance<64, false, FP8, T>(ma, mb, p, grid, stream);
+}
+
+// Whole 16-byte accesses of every array of the output's shape.
+bool epilogue_vec_ok(const LinearEpilogue& ep, int64_t N, const float* planes) {
+  const uintptr_t all = (uintptr_t)ep.out | (uintptr_t)ep.z | (uintptr_t)ep.residual | (uintptr_t)ep.bias |
+                        (uintptr_t)ep.col_scale | (uintptr_t)planes;
+  return N % 8 == 0 && all % 16 == 0;
+}
+
+}  // namespace
+
+size_t linear_tc_workspace(int64_t M, int64_t N, int64_t K, int in_type) {
+  const Plan p = plan_for(M, N, K, in_type);
+  return p.splits > 1 ? (size_t)p.splits * M * N * sizeof(float) + 256 : 0;
+}
+
+int launch_split_epilogue(const float* planes, int parts, int64_t M, int64_t N, const LinearEpilogue& ep, cudaStream_t stream) {
+  const int octs = (int)((N + 7) / 8);
+  const int64_t grid = (M * octs + 255) / 256;
+  const int vec = epilogue_vec_ok(ep, N, planes);
+  if (ep.out_type == GNN_F32) split_epilogue_kernel<float><<<(unsigned)grid, 256, 0, stream>>>(planes, parts, M, (int)N, octs, vec, ep);
+  else if (ep.out_type == GNN_BF16) split_epilogue_kernel<__nv_bfloat16><<<(unsigned)grid, 256, 0, stream>>>(planes, parts, M, (int)N, octs, vec, ep);
+  else split_epilogue_kernel<__half><<<(unsigned)grid, 256, 0, stream>>>(planes, parts, M, (int)N, octs, vec, ep);
+  return GNN_OK;
+}
+
+int launch_linear_tc(const TcOperand& a, const TcOperand& b, int in_type, int64_t M, int64_t N, int64_t K,
+                     const LinearEpilogue& ep, void* workspace, size_t workspace_bytes, int* status, cudaStream_t stream,
+                     const char* what) {
+  const Plan pl = plan_for(M, N, K, in_type);
+  char msg[200];
+  if (pl.splits > 1 && (!workspace || workspace_bytes < linear_tc_workspace(M, N, K, in_type))) {
+    snprintf(msg, sizeof msg, "%s: workspace too small", what);
+    set_last_error(msg);
+    return GNN_ERR_WORKSPACE;
+  }
+  const int64_t tiles = pl.tiles_m * pl.tiles_n * pl.splits;
+  if (tiles > INT32_MAX) {
+    snprintf(msg, sizeof msg, "%s: too many output tiles", what);
+    set_last_error(msg);
+    return GNN_ERR_LIMIT;
+  }
+  CUtensorMap ma, mb;
+  if (!encode(&ma, a, in_type, M, K, BM) || !encode(&mb, b, in_type, N, K, pl.pair ? pl.bn / 2 : pl.bn)) {
+    snprintf(msg, sizeof msg, "%s: cuTensorMapEncodeTiled failed", what);
+    set_last_error(msg);
+    return GNN_ERR_CUDA;
+  }
+  const bool fp8 = in_type == GNN_E4M3;
+  Params p;
+  p.M = (int)M;
+  p.N = (int)N;
+  p.k_elems = fp8 ? kStageK : kStageK / 2;
+  p.total_kb = (int)((K + p.k_elems - 1) / p.k_elems);
+  p.kb_per_split = (p.total_kb + pl.splits - 1) / pl.splits;
+  p.tiles_m = (int)pl.tiles_m;
+  p.tiles_n = (int)pl.tiles_n;
+  p.num_tiles = (int)tiles;
+  p.a_mn = a.mn_major;
+  p.b_mn = b.mn_major;
+  // D = F32 (1 at bits 4-5), A / B type at bits 7-9 / 10-12 (kind f16: 0 half, 1 bfloat16; kind
+  // f8f6f4: 0 e4m3), bit 15 / 16 = A / B is MN-major; N/8 and M/16 are added by the kernel
+  const uint32_t type = in_type == GNN_BF16 ? 1u : 0u;
+  p.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)a.mn_major << 15) | ((uint32_t)b.mn_major << 16);
+  p.planes = pl.splits > 1 ? (float*)(((uintptr_t)workspace + 255) & ~(uintptr_t)255) : nullptr;
+  p.vec_ok = p.planes ? N % 8 == 0 : epilogue_vec_ok(ep, N, nullptr);
+  p.ep = ep;
+  p.status = status;
+  const int64_t units = pl.pair ? kSms / 2 : kSms;
+  const int grid = (int)(tiles < units ? tiles : units) * (pl.pair ? 2 : 1);
+  int rc;
+  if (!fp8) {  // 16-bit operands give results of their own type
+    rc = ep.out_type == GNN_BF16 ? launch_shape<false, __nv_bfloat16>(pl, ma, mb, p, grid, stream)
+                                 : launch_shape<false, __half>(pl, ma, mb, p, grid, stream);
+  } else {
+    rc = ep.out_type == GNN_F32    ? launch_shape<true, float>(pl, ma, mb, p, grid, stream)
+         : ep.out_type == GNN_BF16 ? launch_shape<true, __nv_bfloat16>(pl, ma, mb, p, grid, stream)
+                                   : launch_shape<true, __half>(pl, ma, mb, p, grid, stream);
+  }
+  if (rc == 0 && pl.splits > 1) launch_split_epilogue(p.planes, pl.splits, M, N, ep, stream);
+  return check_launch(what);
+}
+
+}  // namespace gnn

@@ -457,6 +457,7 @@ int gnn_halo_push_ranges(const float* x, int64_t row_floats, const int* send_idx
 #define GNN_F32 0
 #define GNN_BF16 1
 #define GNN_F16 2
+#define GNN_E4M3 3 /* 8-bit operands of gnn_linear_fwd only */
 
 /* Root-mean-square norm of n rows of d elements (1 <= d <= 32768) with the residual's addition:
  *   h = x + residual (NULL: h = x),  rstd = 1 / sqrt(mean(h^2) + eps),  y = h * rstd * weight
@@ -505,6 +506,43 @@ int gnn_expert_combine(const void* rows, const void* weights, const int* slots, 
 int gnn_expert_combine_bwd(const void* grad_out, const void* rows, const void* weights, const int* slots,
                            const int* kept, int dtype, int weight_dtype, int64_t tokens, int k, int64_t width,
                            void* grad_rows, void* grad_weights, cudaStream_t stream);
+
+#define GNN_ACT_NONE 0
+#define GNN_ACT_RELU 1
+#define GNN_ACT_LEAKY_RELU 2
+#define GNN_ACT_ELU 3
+#define GNN_ACT_GELU 4 /* 0.5 z (1 + erf(z / sqrt 2)) */
+#define GNN_ACT_SILU 5
+
+/* Linear layer with bias, activation and residual, x [M,K], w [N,K] (the nn.Linear layout):
+ *   z = x_scale[m] * w_scale[n] * (x w^T) + bias,   y = act(z) + residual
+ * x and w are fp32 (error-compensated 3xTF32, rows K elements apart, K % 4 == 0), bf16, fp16 or
+ * e4m3 (in_type; rows ldx / ldw elements apart, each on a 16-byte boundary); the scales (one per
+ * row of x and of w) belong to e4m3 operands alone.  bias, residual, y and z are of out_type (= in_type
+ * except for e4m3); bias, residual and z may be NULL.  z is what the gradient needs of the forward
+ * pass.  Sums and epilogue are fp32.  `status` as in gnn_gemm_tf32x3. */
+int gnn_linear_fwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int in_type, size_t* bytes);
+int gnn_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int in_type, const float* x_scale,
+                   const float* w_scale, const void* bias, int act, float slope, const void* residual, void* y,
+                   void* z, int out_type, int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes,
+                   int* status, cudaStream_t stream);
+
+/* Elementwise half of its gradient: gz = grad_y * act'(z) (NULL: not wanted; rows ldz >= N elements
+ * apart, the columns behind N set to zero), grad_b = sum over rows of gz (NULL: not wanted; fp32 sums
+ * in a fixed order).  z may be NULL without an activation. */
+int gnn_linear_act_bwd_workspace_bytes(int64_t M, int64_t N, int64_t ldz, size_t* bytes);
+int gnn_linear_act_bwd(const void* grad_y, const void* z, int act, float slope, int dtype, int64_t M, int64_t N,
+                       void* gz, int64_t ldz, void* grad_b, void* workspace, size_t workspace_bytes,
+                       cudaStream_t stream);
+
+/* Its products: grad_x [M,K] = gz w and grad_w [N,K] = gz^T x, fp32, bf16 or fp16; operand rows as
+ * in gnn_linear_fwd (fp32: gz rows N elements apart, for grad_x N % 4 == 0). */
+int gnn_linear_dgrad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, size_t* bytes);
+int gnn_linear_dgrad(const void* gz, int64_t ldg, const void* w, int64_t ldw, int dtype, void* grad_x, int64_t M,
+                     int64_t N, int64_t K, void* workspace, size_t workspace_bytes, int* status, cudaStream_t stream);
+int gnn_linear_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, size_t* bytes);
+int gnn_linear_wgrad(const void* gz, int64_t ldg, const void* x, int64_t ldx, int dtype, void* grad_w, int64_t M,
+                     int64_t N, int64_t K, void* workspace, size_t workspace_bytes, int* status, cudaStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -69,3 +69,52 @@ def test_experts_refuse_cpu_tensors():
         expert_sort(torch.zeros(4, 2, dtype=torch.int32), 3)
     with pytest.raises(TypeError):
         expert_sort([[0]], 3)
+
+
+def test_linear_c_refusals():
+    from ae_mlsys_gnn_b200 import _capi
+
+    lib = _capi.lib()
+    BF16, F32, E4M3 = 1, 0, 3
+
+    def fwd(x=ONE, ldx=64, ldw=64, it=BF16, xs=None, ws=None, act=0, y=ONE, ot=BF16, M=4, N=8, K=64, scratch=None, nb=0,
+            status=ONE):
+        return lib.gnn_linear_fwd(x, ldx, ONE, ldw, it, xs, ws, None, act, 0.2, None, y, None, ot, M, N, K, scratch, nb,
+                                  status, None)
+
+    assert fwd(M=0) == 0
+    assert fwd(x=None) == -1 and fwd(y=None) == -1 and fwd(status=None) == -1
+    assert fwd(M=-1) == -1 and fwd(N=0) == -1 and fwd(K=0) == -1 and fwd(M=1 << 31) == -5
+    assert fwd(act=6) == -1 and fwd(act=-1) == -1
+    assert fwd(it=4) == -4 and fwd(it=BF16, ot=2) == -4 and fwd(it=E4M3, xs=ONE, ws=ONE, ot=3) == -4
+    assert fwd(xs=ONE) == -1 and fwd(it=E4M3) == -1  # scales go with e4m3 operands
+    assert fwd(ldx=60) == -1 and fwd(ldw=63) == -1   # a row shorter than K
+    assert fwd(M=100, ldx=68) == -4 and fwd(M=100, x=ctypes.c_void_p(264)) == -4  # rows off 16-byte boundaries
+    assert fwd(it=F32, ot=F32, ldx=68, M=100) == -4
+    assert fwd(it=F32, ot=F32, K=62, ldx=62, ldw=62, M=100) == -4
+    assert fwd(it=F32, ot=F32, M=100) == -3  # no scratch
+    need = ctypes.c_size_t(0)
+    assert lib.gnn_linear_fwd_workspace_bytes(64, 70, 9000, BF16, ctypes.byref(need)) == 0 and need.value > 0
+    assert fwd(M=64, N=70, K=9000, ldx=9000, ldw=9000) == -3
+    assert lib.gnn_linear_fwd_workspace_bytes(64, 70, 9000, 5, ctypes.byref(need)) == -1
+    act = lambda gy=ONE, z=ONE, a=4, ldz=8, ws=ONE, nb=1 << 20, gz=ONE, gb=ONE, dt=BF16: lib.gnn_linear_act_bwd(
+        gy, z, a, 0.2, dt, 4, 8, gz, ldz, gb, ws, nb, None)
+    assert act(gy=None) == -1 and act(z=None) == -1 and act(gz=None, gb=None) == -1 and act(ldz=7) == -1
+    assert act(ws=None) == -3 and act(dt=3) == -4 and act(a=9) == -1
+    dg = lambda gz=ONE, ldg=8, ldw=64, dt=BF16: lib.gnn_linear_dgrad(gz, ldg, ONE, ldw, dt, ONE, 4, 8, 64, None, 0, ONE, None)
+    wg = lambda gz=ONE, ldg=8, ldx=64, dt=BF16: lib.gnn_linear_wgrad(gz, ldg, ONE, ldx, dt, ONE, 4, 8, 64, None, 0, ONE, None)
+    for f in (dg, wg):
+        assert f(gz=None) == -1 and f(ldg=7) == -1 and f(ldg=12) == -4 and f(dt=3) == -4
+        assert f(dt=F32) == -3 and f(dt=F32, ldg=12) == -4
+
+
+def test_linear_refuses_cpu_tensors():
+    from ae_mlsys_gnn_b200.operators.linear_act import linear_act, linear_act_fp8
+
+    with pytest.raises(ValueError, match="CUDA"):
+        linear_act(torch.zeros(2, 8), torch.zeros(4, 8))
+    with pytest.raises(TypeError):
+        linear_act([0.0], torch.zeros(4, 8))
+    with pytest.raises(ValueError, match="CUDA"):
+        linear_act_fp8(torch.zeros(2, 8).to(torch.float8_e4m3fn), torch.ones(2), torch.zeros(4, 8).to(torch.float8_e4m3fn),
+                       torch.ones(4))
