@@ -168,6 +168,8 @@ using namespace gnn;
 extern "C" int gnn_linear_fwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int in_type, size_t* bytes) {
   if (!bytes || M < 0 || N < 1 || K < 1 || in_type < GNN_F32 || in_type > GNN_E4M3)
     return fail(GNN_ERR_INVALID_ARG, "gnn_linear_fwd_workspace_bytes", "bad argument");
+  *bytes = 0;
+  if (linear_few_wanted(M, N, K, in_type)) return GNN_OK;
   if (in_type == GNN_F32) return gnn_gemm_tf32x3_workspace_bytes(M, N, K, bytes);
   *bytes = linear_tc_workspace(M, N, K, in_type);
   return GNN_OK;
@@ -189,6 +191,10 @@ extern "C" int gnn_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t
   if (ldx < K || ldw < K) return fail(GNN_ERR_INVALID_ARG, what, "a row is shorter than K");
   if (in_type == GNN_F32) {
     if (ldx != K || ldw != K) return fail(GNN_ERR_UNSUPPORTED, what, "fp32 rows must be K elements apart");
+    if (linear_few_wanted(M, N, K, in_type) && K % 4 == 0 && (((uintptr_t)x | (uintptr_t)w) & 15) == 0) {
+      const LinearEpilogue ep{nullptr, nullptr, bias, z, act, slope, residual, y, out_type};
+      return launch_linear_few({x, K, false}, {w, K, false}, in_type, M, N, K, ep, stream, what);
+    }
     const GemmFinish fin{static_cast<const float*>(bias), static_cast<float*>(z), act, slope,
                          static_cast<const float*>(residual)};
     return tf32x3_product(static_cast<const float*>(x), static_cast<const float*>(w), 1, static_cast<float*>(y), M, N, K,
@@ -199,6 +205,7 @@ extern "C" int gnn_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t
   if (!tma_operand_ok(a, elt) || !tma_operand_ok(b, elt))
     return fail(GNN_ERR_UNSUPPORTED, what, "rows must start on 16-byte boundaries");
   const LinearEpilogue ep{x_scale, w_scale, bias, z, act, slope, residual, y, out_type};
+  if (linear_few_wanted(M, N, K, in_type)) return launch_linear_few(a, b, in_type, M, N, K, ep, stream, what);
   return launch_linear_tc(a, b, in_type, M, N, K, ep, workspace, workspace_bytes, status, stream, what);
 }
 

@@ -5,9 +5,13 @@
 // fp32 accumulation in tensor memory, fp32 epilogue, one rounding.  Persistent and warp-specialised:
 //   warp 0      TMA producer: a stage is 128 bytes along the reduction axis of both operands
 //   warp 1      tensor-memory allocation and single-thread tcgen05.mma issue
-//   warps 2-9   epilogue: two warps per 32 rows, alternate 32-column chunks
+//   warps 2-9   epilogue: two warps per 32 rows, alternate units of 32 rows x 128 bytes of output
 // The accumulator is double buffered in tensor memory, so the epilogue of a tile runs under the main
-// loop of the next one.
+// loop of the next one.  A lane of the epilogue owns a row: it reads its sums from tensor memory, adds
+// bias, applies the activation, and writes the rounded row piece into a swizzled 4 KB block of shared
+// memory that TMA stores as whole 128-byte lines (stores straight from registers, 32 or 64 bytes a
+// row, took 2 to 4 us per 64 KB and SM and were the kernel's bound).  The residual arrives in
+// the same block by TMA before the lane replaces it by the result.
 //
 // kPair: two CTAs of a cluster (the two SMs of a TPC) work on one 256 x 256 tile with
 // cta_group::2 MMAs.  Each holds its own 128 rows of A and half of B in shared memory, so a
@@ -26,7 +30,7 @@
 #include "activation.cuh"
 #include "common.cuh"
 #include "dtypes.cuh"
-#include "linear_tc.cuh"
+#include "linear_epilogue.cuh"
 
 namespace gnn {
 namespace {
@@ -37,9 +41,10 @@ constexpr int kATile = BM * kStageK;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 32 * (2 + kEpiWarps);
 constexpr int kMaxStages = 7;
-constexpr int kNumBars = 2 * kMaxStages + 4;
+constexpr int kNumBars = 2 * kMaxStages + 4 + kEpiWarps;
 constexpr int kBarBytes = (8 * kNumBars + 16 + 127) / 128 * 128;
-constexpr int kEpiBytes = kEpiWarps * 32 * 32 * 4;  // a 32 x 32 fp32 block per epilogue warp
+constexpr int kUnitBytes = 32 * 128;                // 32 rows x 128 bytes of output
+constexpr int kSmemLimit = 232448;
 constexpr long long kWaitCycles = 4000000000LL;     // about two seconds
 constexpr long long kDrainCycles = 200000000LL;     // about a tenth of a second
 
@@ -47,10 +52,7 @@ template <int BN, bool PAIR>
 struct Geom {
   static constexpr int kBRows = PAIR ? BN / 2 : BN;  // B rows in this CTA's shared memory
   static constexpr int kStageBytes = kATile + kBRows * kStageK;
-  static constexpr int kFit = (232448 - 1024 - kBarBytes - kEpiBytes) / kStageBytes;
-  static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
   static constexpr int kTmemCols = 2 * BN;
-  static constexpr size_t kSmemBytes = (size_t)kStages * kStageBytes + 1024 + kBarBytes + kEpiBytes;
 };
 
 struct Params {
@@ -61,7 +63,8 @@ struct Params {
   int k_elems;                      // elements of a stage along the reduction axis
   uint32_t idesc;                   // instruction descriptor without the N field
   float* planes;                    // splits > 1: fp32 partial planes [splits][M][N]
-  int vec_ok;                       // whole 16-byte accesses of out, z, residual and bias
+  int stages;
+  int tma_out;                      // out, z, residual (or the planes) have rows that TMA can address
   LinearEpilogue ep;
   int* status;
 };
@@ -100,6 +103,10 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     }
   }
 }
+// The same for a whole warp: all lanes agree on the outcome.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* failed) {
+  return __all_sync(kFull, mbar_wait(bar, parity, failed));
+}
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -121,6 +128,34 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
         ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(bar) : "memory");
 }
+
+__device__ __forceinline__ void tma_load_local(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(c0), "r"(c1), "r"(src)
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(c0), "r"(c1),
+               "r"(c2), "r"(src) : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// The copies out of shared memory issued so far have read it.
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+
+// 16 fp32 columns of tensor memory, one row per lane.
+__device__ __forceinline__ void tmem_load16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // Shared-memory matrix descriptors (version 1, 128-byte swizzle).
 //   K-major tile [rows][128 bytes]: 8-row groups 1024 bytes apart (stride offset), the leading
@@ -188,41 +223,6 @@ __device__ __forceinline__ TileCoord decode_tile(const Params& p, int tile) {
   return t;
 }
 
-// Eight consecutive values of type T at p (16-byte aligned), widened.
-template <class T>
-__device__ __forceinline__ void load8(const T* p, float (&o)[8]) {
-  constexpr int V = 16 / (int)sizeof(T);
-#pragma unroll
-  for (int i = 0; i < 8; i += V) {
-    const Pack<T, V> a = load_pack(reinterpret_cast<const Pack<T, V>*>(p + i));
-#pragma unroll
-    for (int j = 0; j < V; ++j) o[i + j] = to_f32(a.v[j]);
-  }
-}
-template <class T>
-__device__ __forceinline__ void store8(T* p, const float (&o)[8]) {
-  constexpr int V = 16 / (int)sizeof(T);
-#pragma unroll
-  for (int i = 0; i < 8; i += V) {
-    Pack<T, V> a;
-#pragma unroll
-    for (int j = 0; j < V; ++j) a.v[j] = from_f32<T>(o[i + j]);
-    store_pack(reinterpret_cast<Pack<T, V>*>(p + i), a);
-  }
-}
-
-// The epilogue of one element, for outputs whose rows are not whole 16-byte units.
-template <class T>
-__device__ __forceinline__ void finish_one(const LinearEpilogue& ep, int64_t row, int col, int N, float v) {
-  const int64_t at = row * N + col;
-  if (ep.col_scale) v *= __ldg(ep.row_scale + row) * __ldg(ep.col_scale + col);
-  if (ep.bias) v += to_f32(static_cast<const T*>(ep.bias)[col]);
-  if (ep.z) static_cast<T*>(ep.z)[at] = from_f32<T>(v);
-  v = act_value<sizeof(T) == 4>(v, ep.act, ep.slope);
-  if (ep.residual) v += to_f32(static_cast<const T*>(ep.residual)[at]);
-  static_cast<T*>(ep.out)[at] = from_f32<T>(v);
-}
-
 // Eight columns of kRows rows at a time: residual, bias and scales are requested early, and the
 // activation is one branch for all 8 * kRows values.
 template <class T, int kRows>
@@ -287,23 +287,53 @@ struct Finish8 {
   }
 };
 
+// Sixteen consecutive columns of one output row in a unit's block: the 16-byte units of row r are
+// exchanged by r mod 8 (the pattern of TMA's 128-byte swizzle), so 8 lanes on 8 rows meet 8 banks.
+template <class O>
+struct RowPiece {
+  static constexpr int V = 16 / (int)sizeof(O), kUnits = 16 / V;  // 16-byte units of 16 columns
+  __device__ __forceinline__ static uint8_t* at(uint8_t* block, int lane, int piece, int u) {
+    return block + lane * 128 + (((piece * kUnits + u) ^ (lane & 7)) << 4);
+  }
+  __device__ __forceinline__ static void put(uint8_t* block, int lane, int piece, const float (&v)[16]) {
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      Pack<O, V> o;
+#pragma unroll
+      for (int j = 0; j < V; ++j) o.v[j] = from_f32<O>(v[u * V + j]);
+      store_pack(reinterpret_cast<Pack<O, V>*>(at(block, lane, piece, u)), o);
+    }
+  }
+  __device__ __forceinline__ static void add(uint8_t* block, int lane, int piece, float (&v)[16]) {
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const Pack<O, V> o = load_pack(reinterpret_cast<const Pack<O, V>*>(at(block, lane, piece, u)));
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[u * V + j] += to_f32(o.v[j]);
+    }
+  }
+};
+
 template <int BN, bool PAIR, bool FP8, class T>
 __global__ void __launch_bounds__(kThreads, 1)
-linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
+linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                 const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_z,
+                 const __grid_constant__ CUtensorMap map_res, const Params p) {
   using G = Geom<BN, PAIR>;
-  constexpr int kStages = G::kStages;
   constexpr int TM = PAIR ? 2 * BM : BM;
   extern __shared__ uint8_t smem_raw[];
+  const int stages = p.stages;
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t base = (raw_addr + 1023u) & ~1023u;  // swizzle atoms need 1024-byte alignment
   uint8_t* const base_ptr = smem_raw + (base - raw_addr);
-  const uint32_t bars = base + kStages * G::kStageBytes;
+  const uint32_t bar_off = stages * G::kStageBytes + kEpiWarps * kUnitBytes * (p.ep.z ? 2 : 1);
+  const uint32_t bars = base + bar_off;
   auto full_bar = [&](int s) { return bars + 8u * s; };                             // TMA -> MMA
   auto empty_bar = [&](int s) { return bars + 8u * (kMaxStages + s); };             // MMA -> TMA
   auto acc_full_bar = [&](int b) { return bars + 8u * (2 * kMaxStages + b); };      // MMA -> epilogue
   auto acc_empty_bar = [&](int b) { return bars + 8u * (2 * kMaxStages + 2 + b); }; // epilogue -> MMA
+  auto res_bar = [&](int w) { return bars + 8u * (2 * kMaxStages + 4 + w); };       // residual -> its epilogue warp
   const uint32_t tmem_slot = bars + 8u * kNumBars;
-  float4* const epi = reinterpret_cast<float4*>(base_ptr + kStages * G::kStageBytes + kBarBytes);
 
   __shared__ volatile int s_failed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -312,7 +342,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 
   if (threadIdx.x == 0) {
     s_failed = 0;
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < stages; ++s) {
       mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), 1);
     }
@@ -320,6 +350,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       mbar_init(acc_full_bar(b), 1);
       mbar_init(acc_empty_bar(b), kEpiWarps * (PAIR ? 2 : 1));
     }
+    for (int w = 0; w < kEpiWarps; ++w) mbar_init(res_bar(w), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -335,19 +366,18 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   __syncthreads();
   if constexpr (PAIR) cluster_sync();  // the other CTA's barriers exist
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(base_ptr + kStages * G::kStageBytes + 8 * kNumBars);
+  const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(base_ptr + bar_off + 8 * kNumBars);
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer
     if (lane == 0) {
-      uint32_t it = 0;
+      int s = 0;
+      uint32_t phase = 1;  // a fresh barrier lets the wait for parity 1 through
       for (int tile = unit; tile < p.num_tiles && !s_failed; tile += units) {
         const TileCoord t = decode_tile<TM, BN>(p, tile);
         const int a_row = t.m0 + (int)rank * BM, b_row = t.n0 + (int)rank * G::kBRows;
-        for (int kb = 0; kb < t.num_kb; ++kb, ++it) {
-          const int s = it % kStages;
-          const uint32_t round = it / kStages;
-          if (round > 0 && !mbar_wait(empty_bar(s), (round - 1) & 1, &s_failed)) { s_failed = 1; break; }
+        for (int kb = 0; kb < t.num_kb; ++kb) {
+          if (!mbar_wait(empty_bar(s), phase, &s_failed)) { s_failed = 1; break; }
           const uint32_t st = base + s * G::kStageBytes;
           const int k0 = (t.kb_begin + kb) * p.k_elems;
           if (rank == 0) mbar_expect_tx(full_bar(s), G::kStageBytes * (PAIR ? 2 : 1));
@@ -364,6 +394,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           } else {
             tma_load<PAIR>(st + kATile, &map_b, k0, b_row, full_bar(s));
           }
+          if (++s == stages) { s = 0; phase ^= 1; }
         }
       }
     }
@@ -373,109 +404,173 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       const uint64_t a_step = p.a_mn ? (2048 >> 4) : (32 >> 4);  // descriptor advance per K slice
       const uint64_t b_step = p.b_mn ? (2048 >> 4) : (32 >> 4);
       const uint32_t idesc = p.idesc | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
-      uint32_t it = 0, count = 0;
+      int s = 0;
+      uint32_t phase = 0, count = 0;
       bool ok = true;
       for (int tile = unit; tile < p.num_tiles && ok && !s_failed; tile += units, ++count) {
         const TileCoord t = decode_tile<TM, BN>(p, tile);
         const int buf = count & 1;
-        // a fresh barrier lets the wait for parity 1 through: the first use of a buffer does not block
         if (!mbar_wait(acc_empty_bar(buf), ((count >> 1) & 1) ^ 1, &s_failed)) { s_failed = 1; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t acc = tmem_base + (uint32_t)(buf * BN);
-        for (int kb = 0; kb < t.num_kb; ++kb, ++it) {
-          const int s = it % kStages;
-          if (!mbar_wait(full_bar(s), (it / kStages) & 1, &s_failed)) { s_failed = 1; ok = false; break; }
+        for (int kb = 0; kb < t.num_kb; ++kb) {
+          if (!mbar_wait(full_bar(s), phase, &s_failed)) { s_failed = 1; ok = false; break; }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t st = base + s * G::kStageBytes;
           const uint64_t da = operand_desc(st, p.a_mn), db = operand_desc(st + kATile, p.b_mn);
 #pragma unroll
           for (int k = 0; k < 4; ++k) umma<PAIR, FP8>(acc, da + a_step * k, db + b_step * k, idesc, (kb | k) != 0);
           umma_commit<PAIR>(empty_bar(s));  // the stage is free once these MMAs have read it
+          if (++s == stages) { s = 0; phase ^= 1; }
         }
         if (ok) umma_commit<PAIR>(acc_full_bar(buf));
       }
     }
   } else {
     // ---------------------------------------------------------------- epilogue
-    const int lg = warp & 3;            // this warp may touch tensor-memory lanes [32*lg, 32*lg + 32)
-    const int half = (warp - 2) >> 2;   // even or odd 32-column chunks
-    float4* const stg = epi + (warp - 2) * 256;
-    const int sub = lane >> 2, oct = lane & 3;  // row of 8 and 8-column group this lane finishes
-    uint32_t count = 0;
+    const int w = warp - 2;
+    const int lg = warp & 3;   // this warp may touch tensor-memory lanes [32*lg, 32*lg + 32)
+    const int part = w >> 2;   // units part, part + 2, ... of its rows
+    uint8_t* const block = base_ptr + stages * G::kStageBytes + w * kUnitBytes;
+    uint8_t* const z_block = block + kEpiWarps * kUnitBytes;
+    const bool with_res = p.tma_out && p.ep.residual && !p.planes;
+    uint32_t res_phase = 0, count = 0;
+    bool res_due = false;  // a residual copy is under way (lane 0's view)
+
     for (int tile = unit; tile < p.num_tiles && !s_failed; tile += units, ++count) {
       const TileCoord t = decode_tile<TM, BN>(p, tile);
       const int buf = count & 1;
-      const int64_t row0 = t.m0 + (int)rank * BM + lg * 32 + sub;  // this lane's rows: row0 + 8 i
-      Finish8<T, 4> fin;
-      const bool whole = p.vec_ok && !p.planes;
-      auto in = [&](int col) { return [=](int i) { return row0 + 8 * i < p.M && col < p.N; }; };
-      if (whole) {  // the first chunk's residual is under way while the product finishes
-        const int col = t.n0 + half * 32 + oct * 8;
-        fin.request(p.ep, row0, 8, col, p.N, in(col));
-      }
-      if (!mbar_wait(acc_full_bar(buf), (count >> 1) & 1, &s_failed)) { s_failed = 1; break; }
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll 1
-      for (int c = half; c < BN / 32; c += 2) {
-        const int col0 = t.n0 + c * 32;
-        if (col0 >= p.N) break;
-        uint32_t r[32];
-        const uint32_t taddr = tmem_base + ((uint32_t)(lg * 32) << 16) + (uint32_t)(buf * BN + c * 32);
-        asm volatile(
-            "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-            "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-            "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-              "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-              "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-              "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-            : "r"(taddr) : "memory");
-        const int col = col0 + oct * 8;
-        if (whole) fin.columns(p.ep, row0, 8, col, col < p.N, in(col));
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if (t.num_kb == 0) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) r[j] = 0u;  // an empty range contributes nothing
+      const int top = t.m0 + (int)rank * BM + lg * 32;  // first row of this warp
+      const int row = top + lane;
+
+      // The units of this warp's rows, of output type O (fp32 for planes).
+      auto run = [&](auto tag, auto is_plane) -> bool {
+        using O = decltype(tag);
+        using Piece = RowPiece<O>;
+        constexpr bool kPlanes = decltype(is_plane)::value;
+        constexpr int kCols = 128 / (int)sizeof(O), kPieces = kCols / 16;
+        auto want_residual = [&](int col0) {  // the block is free: its last store has been read
+          if (lane == 0) {
+            mbar_expect_tx(res_bar(w), kUnitBytes);
+            tma_load_local(base + stages * G::kStageBytes + w * kUnitBytes, &map_res, col0, top, res_bar(w));
+            res_due = true;
+          }
+        };
+        const bool mine = top < p.M && part * kCols < BN && t.n0 + part * kCols < p.N;
+        if (mine && !kPlanes && with_res) {  // the first residual is under way while the product finishes
+          if (lane == 0) bulk_wait_read();
+          want_residual(t.n0 + part * kCols);
         }
-        // Through shared memory from one row per lane to four lanes per row, so that a warp
-        // instruction covers 64-byte pieces of 8 rows; the 16-byte units of row r are rotated by
-        // r mod 8, which keeps both sides free of bank conflicts.
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          stg[lane * 8 + (j ^ (lane & 7))] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
-                                                         __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
-        __syncwarp();
-        if (p.vec_ok) {
-          float v[32];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int rr = i * 8 + sub;
-            const float4 lo = stg[rr * 8 + ((oct * 2) ^ (rr & 7))], hi = stg[rr * 8 + ((oct * 2 + 1) ^ (rr & 7))];
-            v[8 * i] = lo.x; v[8 * i + 1] = lo.y; v[8 * i + 2] = lo.z; v[8 * i + 3] = lo.w;
-            v[8 * i + 4] = hi.x; v[8 * i + 5] = hi.y; v[8 * i + 6] = hi.z; v[8 * i + 7] = hi.w;
-          }
-          if (whole) {
-            fin.finish(p.ep, row0, 8, col, p.N, in(col), v);
-            if (c + 2 < BN / 32) fin.request(p.ep, row0, 8, col + 64, p.N, in(col + 64));
+        const float rs = !kPlanes && p.ep.col_scale && row < p.M ? __ldg(p.ep.row_scale + row) : 1.f;
+        if (!warp_wait(acc_full_bar(buf), (count >> 1) & 1, &s_failed)) return false;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (!mine) return true;
+        const uint32_t lane_base = tmem_base + ((uint32_t)(lg * 32) << 16) + (uint32_t)(buf * BN);
+#pragma unroll 1
+        for (int u = part; u < BN / kCols; u += 2) {
+          const int col0 = t.n0 + u * kCols;
+          if (col0 >= p.N) break;
+          if (!kPlanes && with_res) {
+            if (!warp_wait(res_bar(w), res_phase, &s_failed)) return false;
+            res_phase ^= 1;
+            if (lane == 0) res_due = false;
           } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (in(col)(i)) Finish8<float, 4>::store_row(p.planes + ((size_t)t.z * p.M + row0 + 8 * i) * p.N + col, v, i);
+            if (lane == 0) bulk_wait_read();
+            __syncwarp();
           }
-        } else {
-          // one element per lane and step: neighbours of a row on neighbouring lanes
-          const float* const flat = reinterpret_cast<const float*>(stg);
-          const int64_t top = t.m0 + (int)rank * BM + lg * 32;
+#pragma unroll 1
+          for (int q = 0; q < kPieces; ++q) {
+            uint32_t r[16];
+            tmem_load16(lane_base + (uint32_t)(u * kCols + q * 16), r);
+            const int col = col0 + q * 16;
+            float v[16], b[16];
+            const bool in = col + 16 <= p.N;
+            if (!kPlanes && p.ep.bias) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                float f[8];
+                if (in) {
+                  load8(static_cast<const T*>(p.ep.bias) + col + 8 * h, f);
+                } else {
+#pragma unroll
+                  for (int j = 0; j < 8; ++j)
+                    f[j] = col + 8 * h + j < p.N ? to_f32(static_cast<const T*>(p.ep.bias)[col + 8 * h + j]) : 0.f;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) b[8 * h + j] = f[j];
+              }
+            }
+            tmem_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = t.num_kb ? __uint_as_float(r[j]) : 0.f;  // an empty range adds nothing
+            if constexpr (!kPlanes) {
+              if constexpr (FP8) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] *= rs * (in || col + j < p.N ? __ldg(p.ep.col_scale + col + j) : 0.f);
+              }
+              if (p.ep.bias) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] += b[j];
+              }
+              if (p.ep.z) Piece::put(z_block, lane, q, v);
+              apply_act<sizeof(O) == 4>(v, p.ep.act, p.ep.slope);
+              if (with_res) Piece::add(block, lane, q, v);
+            }
+            Piece::put(block, lane, q, v);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            const uint32_t src = base + stages * G::kStageBytes + w * kUnitBytes;
+            if constexpr (kPlanes) {
+              tma_store_3d(&map_out, src, col0, top, t.z);
+            } else {
+              tma_store_2d(&map_out, src, col0, top);
+              if (p.ep.z) tma_store_2d(&map_z, src + kEpiWarps * kUnitBytes, col0, top);
+            }
+            bulk_commit();
+          }
+          if (!kPlanes && with_res && u + 2 < BN / kCols && col0 + 2 * kCols < p.N) {
+            if (lane == 0) bulk_wait_read();
+            want_residual(col0 + 2 * kCols);
+          }
+        }
+        return true;
+      };
+
+      if (p.tma_out) {
+        const bool ok = p.planes ? run(float{}, std::true_type{}) : run(T{}, std::false_type{});
+        if (!ok) { s_failed = 1; break; }
+      } else {
+        // rows that are not whole 16-byte units: 32 x 32 blocks through shared memory, then one element
+        // per lane and step, neighbours of a row on neighbouring lanes
+        if (!warp_wait(acc_full_bar(buf), (count >> 1) & 1, &s_failed)) { s_failed = 1; break; }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+        for (int c = part; c < BN / 32; c += 2) {
+          const int col0 = t.n0 + c * 32;
+          if (col0 >= p.N || top >= p.M) break;
+#pragma unroll 1
+          for (int q = 0; q < 2; ++q) {
+            uint32_t r[16];
+            tmem_load16(tmem_base + ((uint32_t)(lg * 32) << 16) + (uint32_t)(buf * BN + c * 32 + q * 16), r);
+            tmem_wait();
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = t.num_kb ? __uint_as_float(r[j]) : 0.f;
+            RowPiece<float>::put(block, lane, q, v);
+          }
+          __syncwarp();
           if (col0 + lane < p.N) {
 #pragma unroll 1
             for (int rr = 0; rr < 32 && top + rr < p.M; ++rr) {
-              const float v = flat[(rr * 8 + ((lane >> 2) ^ (rr & 7))) * 4 + (lane & 3)];
+              const float v = *reinterpret_cast<const float*>(block + rr * 128 + (((lane >> 2) ^ (rr & 7)) << 4) + (lane & 3) * 4);
               if (p.planes) p.planes[((size_t)t.z * p.M + top + rr) * p.N + col0 + lane] = v;
               else finish_one<T>(p.ep, top + rr, col0 + lane, p.N, v);
             }
           }
+          __syncwarp();  // the block is rewritten by the next chunk
         }
-        __syncwarp();  // the block is rewritten by the next chunk
       }
       // the buffer may be overwritten once every epilogue warp has read it
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -484,6 +579,10 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         if constexpr (PAIR) mbar_arrive_at(acc_empty_bar(buf), 0);
         else mbar_arrive(acc_empty_bar(buf));
       }
+    }
+    if (lane == 0) {
+      bulk_wait_read();  // the stores have left shared memory
+      if (s_failed && res_due) mbar_wait(res_bar(w), res_phase, nullptr, kDrainCycles);
     }
   }
 
@@ -494,7 +593,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     // memory is released
     if (threadIdx.x == 0) {
       *p.status = 1;
-      for (int s = 0; s < kStages; ++s) {
+      for (int s = 0; s < stages; ++s) {
         mbar_wait(full_bar(s), 0, nullptr, kDrainCycles);
         mbar_wait(full_bar(s), 1, nullptr, kDrainCycles);
       }
@@ -581,41 +680,77 @@ bool encode(CUtensorMap* m, const TcOperand& o, int in_type, int64_t rows, int64
          CUDA_SUCCESS;
 }
 
+// Map over an output-shaped array [planes][M][N] with a box of 32 rows x 128 bytes.
+bool encode_out(CUtensorMap* m, const void* ptr, int type, int64_t planes, int64_t M, int64_t N) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const int elt = dtype_bytes(type);
+  const CUtensorMapDataType dt = type == GNN_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : type == GNN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                    : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  cuuint64_t dims[3] = {(cuuint64_t)N, (cuuint64_t)M, (cuuint64_t)(planes ? planes : 1)};
+  cuuint64_t strides[2] = {(cuuint64_t)N * elt, (cuuint64_t)M * N * elt};
+  cuuint32_t box[3] = {(cuuint32_t)(128 / elt), 32, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return fn(m, dt, planes ? 3 : 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 struct Plan {
   int bn, pair, splits;
   int64_t tiles_m, tiles_n;
 };
 constexpr int kSms = 148;
 
-// Tile and split of the reduction axis for a shape.
+// Tile and split of the reduction axis for a shape: the candidate with the least estimated time.
+// A stage costs its shared-memory traffic (every operand byte is written by TMA and read by the MMAs,
+// 128 bytes a cycle) or its MMAs, whichever is more; a tile costs about kTileCycles on top that a wave
+// cannot hide, a split a second pass over fp32 planes.
 Plan plan_for(int64_t M, int64_t N, int64_t K, int in_type) {
   const int64_t kb = (K * (in_type == GNN_E4M3 ? 1 : 2) + kStageK - 1) / kStageK;
-  Plan p;
-  auto tiles = [&](int tm, int tn) { return ((M + tm - 1) / tm) * ((N + tn - 1) / tn); };
-  p.pair = M > BM && tiles(256, 256) >= kSms / 2;
-  p.bn = p.pair ? 256 : (tiles(128, 128) >= kSms || N > 64 ? 128 : 64);
-  const int tm = p.pair ? 256 : 128;
-  p.tiles_m = (M + tm - 1) / tm;
-  p.tiles_n = (N + p.bn - 1) / p.bn;
-  const int64_t units = p.pair ? kSms / 2 : kSms, t = p.tiles_m * p.tiles_n;
-  int64_t s = units / t;              // fill the GPU
-  if (s > kb / 8) s = kb / 8;         // at least 8 stages a range
+  struct { int bn, pair; double stage; } const shapes[] = {
+      {256, 1, 512}, {128, 1, 384}, {128, 0, 512}, {64, 0, 384}};
+  constexpr double kTileCycles = 5000, kSplitCycles = 6000, kPlaneBytesPerCycle = 3000;
   // the tensor cores add with truncation (about 2^-26 a step): no chain of more than 2048 stages
   const int64_t least = (kb + 2047) / 2048;
-  if (s < least) s = least;
-  p.splits = s < 1 ? 1 : (int)s;
-  return p;
+  Plan best{};
+  double best_cost = 0;
+  for (const auto& c : shapes) {
+    if (c.pair ? M <= BM : M > BM && N > 64) continue;  // a pair's second half would be empty; a pair reads less
+    const int64_t tm = c.pair ? 2 * BM : BM, units = c.pair ? kSms / 2 : kSms;
+    const int64_t tiles_m = (M + tm - 1) / tm, tiles_n = (N + c.bn - 1) / c.bn, tiles = tiles_m * tiles_n;
+    for (int64_t s = 1; s <= 64; s *= 2) {
+      if (s > 1 && (kb / s < 4 || tiles * s > 2 * units) && s > least) break;
+      if (s < least && s * 2 <= 64) continue;
+      const double waves = (double)((tiles * s + units - 1) / units), stages = (double)((kb + s - 1) / s);
+      const double cost = waves * (stages * c.stage + kTileCycles) +
+                          (s > 1 ? kSplitCycles + 8.0 * s * M * N / kPlaneBytesPerCycle : 0);
+      if (best_cost == 0 || cost < best_cost) {
+        best_cost = cost;
+        best = Plan{c.bn, c.pair, (int)(s < least ? least : s), tiles_m, tiles_n};
+      }
+    }
+  }
+  return best;
 }
 
+struct Maps {
+  CUtensorMap a, b, out, z, res;
+};
+
 template <int BN, bool PAIR, bool FP8, class T>
-int launch_instance(const CUtensorMap& ma, const CUtensorMap& mb, const Params& p, int grid, cudaStream_t stream) {
+int launch_instance(const Maps& m, Params p, int grid, cudaStream_t stream) {
   using G = Geom<BN, PAIR>;
   auto kernel = linear_tc_kernel<BN, PAIR, FP8, T>;
-  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)G::kSmemBytes);
+  const int fixed = 1024 + kBarBytes + kEpiWarps * kUnitBytes * (p.ep.z ? 2 : 1);
+  p.stages = (kSmemLimit - 64 - fixed) / G::kStageBytes;
+  if (p.stages > kMaxStages) p.stages = kMaxStages;
+  const int smem = fixed + p.stages * G::kStageBytes;
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = G::kSmemBytes;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -624,14 +759,15 @@ int launch_instance(const CUtensorMap& ma, const CUtensorMap& mb, const Params& 
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, ma, mb, p) == cudaSuccess ? 0 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, m.a, m.b, m.out, m.z, m.res, p) == cudaSuccess ? 0 : 1;
 }
 
 template <bool FP8, class T>
-int launch_shape(const Plan& pl, const CUtensorMap& ma, const CUtensorMap& mb, const Params& p, int grid, cudaStream_t stream) {
-  if (pl.pair) return launch_instance<256, true, FP8, T>(ma, mb, p, grid, stream);
-  if (pl.bn == 128) return launch_instance<128, false, FP8, T>(ma, mb, p, grid, stream);
-  return launch_instance<64, false, FP8, T>(ma, mb, p, grid, stream);
+int launch_shape(const Plan& pl, const Maps& m, const Params& p, int grid, cudaStream_t stream) {
+  if (pl.pair && pl.bn == 256) return launch_instance<256, true, FP8, T>(m, p, grid, stream);
+  if (pl.pair) return launch_instance<128, true, FP8, T>(m, p, grid, stream);
+  if (pl.bn == 128) return launch_instance<128, false, FP8, T>(m, p, grid, stream);
+  return launch_instance<64, false, FP8, T>(m, p, grid, stream);
 }
 
 // Whole 16-byte accesses of every array of the output's shape.
@@ -674,14 +810,27 @@ int launch_linear_tc(const TcOperand& a, const TcOperand& b, int in_type, int64_
     set_last_error(msg);
     return GNN_ERR_LIMIT;
   }
-  CUtensorMap ma, mb;
-  if (!encode(&ma, a, in_type, M, K, BM) || !encode(&mb, b, in_type, N, K, pl.pair ? pl.bn / 2 : pl.bn)) {
+  Maps m = {};
+  float* const planes = pl.splits > 1 ? (float*)(((uintptr_t)workspace + 255) & ~(uintptr_t)255) : nullptr;
+  // the epilogue goes through TMA where rows are a multiple of 16 bytes apart and start on such a boundary
+  const uintptr_t arrays = planes ? (uintptr_t)planes
+                                  : (uintptr_t)ep.out | (uintptr_t)ep.z | (uintptr_t)ep.residual | (uintptr_t)ep.bias;
+  const bool tma_out = N * (planes ? 4 : dtype_bytes(ep.out_type)) % 16 == 0 && arrays % 16 == 0;
+  bool encoded = encode(&m.a, a, in_type, M, K, BM) && encode(&m.b, b, in_type, N, K, pl.pair ? pl.bn / 2 : pl.bn);
+  if (encoded && tma_out && planes) {
+    encoded = encode_out(&m.out, planes, GNN_F32, pl.splits, M, N);
+  } else if (encoded && tma_out) {
+    encoded = encode_out(&m.out, ep.out, ep.out_type, 0, M, N);
+    if (ep.z) encoded = encoded && encode_out(&m.z, ep.z, ep.out_type, 0, M, N);
+    if (ep.residual) encoded = encoded && encode_out(&m.res, ep.residual, ep.out_type, 0, M, N);
+  }
+  if (!encoded) {
     snprintf(msg, sizeof msg, "%s: cuTensorMapEncodeTiled failed", what);
     set_last_error(msg);
     return GNN_ERR_CUDA;
   }
   const bool fp8 = in_type == GNN_E4M3;
-  Params p;
+  Params p = {};
   p.M = (int)M;
   p.N = (int)N;
   p.k_elems = fp8 ? kStageK : kStageK / 2;
@@ -696,20 +845,21 @@ int launch_linear_tc(const TcOperand& a, const TcOperand& b, int in_type, int64_
   // f8f6f4: 0 e4m3), bit 15 / 16 = A / B is MN-major; N/8 and M/16 are added by the kernel
   const uint32_t type = in_type == GNN_BF16 ? 1u : 0u;
   p.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)a.mn_major << 15) | ((uint32_t)b.mn_major << 16);
-  p.planes = pl.splits > 1 ? (float*)(((uintptr_t)workspace + 255) & ~(uintptr_t)255) : nullptr;
-  p.vec_ok = p.planes ? N % 8 == 0 : epilogue_vec_ok(ep, N, nullptr);
+  p.planes = planes;
+  p.tma_out = tma_out;
   p.ep = ep;
+  if (planes) p.ep.z = nullptr;  // the second kernel writes it
   p.status = status;
   const int64_t units = pl.pair ? kSms / 2 : kSms;
   const int grid = (int)(tiles < units ? tiles : units) * (pl.pair ? 2 : 1);
   int rc;
   if (!fp8) {  // 16-bit operands give results of their own type
-    rc = ep.out_type == GNN_BF16 ? launch_shape<false, __nv_bfloat16>(pl, ma, mb, p, grid, stream)
-                                 : launch_shape<false, __half>(pl, ma, mb, p, grid, stream);
+    rc = ep.out_type == GNN_BF16 ? launch_shape<false, __nv_bfloat16>(pl, m, p, grid, stream)
+                                 : launch_shape<false, __half>(pl, m, p, grid, stream);
   } else {
-    rc = ep.out_type == GNN_F32    ? launch_shape<true, float>(pl, ma, mb, p, grid, stream)
-         : ep.out_type == GNN_BF16 ? launch_shape<true, __nv_bfloat16>(pl, ma, mb, p, grid, stream)
-                                   : launch_shape<true, __half>(pl, ma, mb, p, grid, stream);
+    rc = ep.out_type == GNN_F32    ? launch_shape<true, float>(pl, m, p, grid, stream)
+         : ep.out_type == GNN_BF16 ? launch_shape<true, __nv_bfloat16>(pl, m, p, grid, stream)
+                                   : launch_shape<true, __half>(pl, m, p, grid, stream);
   }
   if (rc == 0 && pl.splits > 1) launch_split_epilogue(p.planes, pl.splits, M, N, ep, stream);
   return check_launch(what);

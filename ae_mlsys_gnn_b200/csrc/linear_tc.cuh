@@ -37,6 +37,12 @@ size_t linear_tc_workspace(int64_t M, int64_t N, int64_t K, int in_type);
 int launch_split_epilogue(const float* planes, int parts, int64_t M, int64_t N, const LinearEpilogue& ep,
                           cudaStream_t stream);
 
+// The same product for few rows (linear_few.cu), bound by the bytes of B: no workspace, no status.
+// fp32 operands too (rows K elements apart, K % 4 == 0).
+bool linear_few_wanted(int64_t M, int64_t N, int64_t K, int in_type);
+int launch_linear_few(const TcOperand& a, const TcOperand& b, int in_type, int64_t M, int64_t N, int64_t K,
+                      const LinearEpilogue& ep, cudaStream_t stream, const char* what);
+
 // TMA reads an operand whose rows are a multiple of 16 bytes apart and 16-byte aligned.
 inline bool tma_operand_ok(const TcOperand& o, int elt) {
   return (reinterpret_cast<uintptr_t>(o.p) & 15) == 0 && o.ld * elt % 16 == 0;
