@@ -10,7 +10,8 @@
 // agree, so a lane loads 16 consecutive bytes of a row and feeds them to two MMAs as they lie: no
 // shared memory, no shuffles between load and MMA.  (tcgen05 would need the operands in shared memory
 // and 128 rows of output; its rate is not what bounds this shape.)
-// fp32: multiply-adds, lanes along the reduction axis.
+// fp32: multiply-adds, lanes along the reduction axis, 4 or 8 rows a CTA (the row groups beyond the
+// first find W in L2).
 #include <stdio.h>
 #include "common.cuh"
 #include "linear_epilogue.cuh"
@@ -110,7 +111,7 @@ __device__ __forceinline__ void join_and_finish(const LinearEpilogue& ep, float*
 
 // NT tiles of 16 columns, MG groups of 8 rows; U pieces of 64 bytes of every row are requested at once.
 template <int KIND, int MG, int NT, int U>
-__global__ void __launch_bounds__(32 * kWarps) few_mma_kernel(const FewParams p) {
+__global__ void __launch_bounds__(32 * kWarps, 4) few_mma_kernel(const FewParams p) {
   __shared__ float parts[kWarps * MG * 8 * NT * 16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int col0 = blockIdx.x * (16 * NT);
@@ -191,6 +192,7 @@ __global__ void __launch_bounds__(32 * kWarps) few_mma_kernel(const FewParams p)
 template <int COLS, int ROWS>
 __global__ void __launch_bounds__(32 * kWarps) few_fma_kernel(const FewParams p) {
   static_assert(COLS * ROWS == 32, "32 sums a lane");
+  const int first = blockIdx.z * ROWS, rows = min(ROWS, p.M - first);
   __shared__ float parts[kWarps * 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int col0 = blockIdx.x * COLS;
@@ -207,7 +209,7 @@ __global__ void __launch_bounds__(32 * kWarps) few_fma_kernel(const FewParams p)
       w[c] = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
     }
 #pragma unroll
-    for (int m = 0; m < ROWS; ++m) x[m] = __ldg(reinterpret_cast<const float4*>(p.x + (int64_t)min(m, p.M - 1) * p.ldx + k));
+    for (int m = 0; m < ROWS; ++m) x[m] = __ldg(reinterpret_cast<const float4*>(p.x + (int64_t)(first + min(m, rows - 1)) * p.ldx + k));
 #pragma unroll
     for (int m = 0; m < ROWS; ++m)
 #pragma unroll
@@ -219,7 +221,7 @@ __global__ void __launch_bounds__(32 * kWarps) few_fma_kernel(const FewParams p)
   }
   warp_multi_sum<32>(acc, lane);  // lane i holds sum i
   parts[warp * 32 + lane] = acc[0];
-  join_and_finish(p.ep, parts, 32, COLS, p.M, p.N, 0, col0);
+  join_and_finish(p.ep, parts, 32, COLS, p.M, p.N, first, col0);
 }
 
 // CTAs along the reduction axis (a cluster): enough of them that the GPU is full, as long as every
@@ -231,9 +233,9 @@ int cluster_for(int64_t col_ctas, int64_t blocks) {
 }
 
 template <class Kernel>
-bool launch(Kernel kernel, int64_t col_ctas, int cluster, const FewParams& p, cudaStream_t stream) {
+bool launch(Kernel kernel, int64_t col_ctas, int cluster, const FewParams& p, cudaStream_t stream, int row_groups = 1) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)col_ctas, (unsigned)cluster);
+  cfg.gridDim = dim3((unsigned)col_ctas, (unsigned)cluster, (unsigned)row_groups);
   cfg.blockDim = dim3(32 * kWarps);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -248,21 +250,15 @@ bool launch(Kernel kernel, int64_t col_ctas, int cluster, const FewParams& p, cu
 
 template <int KIND>
 void launch_kind(const FewParams& p, cudaStream_t stream) {
-  if (p.M <= 8) {
-    const int64_t ctas = (p.N + 15) / 16;
-    launch(few_mma_kernel<KIND, 1, 1, 4>, ctas, cluster_for(ctas, (p.row_bytes + 255) / 256), p, stream);
-  } else if (p.M <= 16) {
-    const int64_t ctas = (p.N + 31) / 32;
-    launch(few_mma_kernel<KIND, 2, 2, 2>, ctas, cluster_for(ctas, (p.row_bytes + 127) / 128), p, stream);
-  } else {
-    const int64_t ctas = (p.N + 31) / 32;
-    launch(few_mma_kernel<KIND, 4, 2, 2>, ctas, cluster_for(ctas, (p.row_bytes + 127) / 128), p, stream);
-  }
+  const int64_t ctas = (p.N + 15) / 16;
+  launch(few_mma_kernel<KIND, 1, 1, 4>, ctas, cluster_for(ctas, (p.row_bytes + 255) / 256), p, stream);
 }
 
 }  // namespace
 
-bool linear_few_wanted(int64_t M, int64_t N, int64_t K, int in_type) { return M <= (in_type == GNN_F32 ? 8 : 32); }
+// fp32: the 3xTF32 kernel splits W into a workspace first, three passes over it, which pays from about
+// 64 rows on (33 rows, N = 8192, K = 4096: 222 us against 47 us per 8 rows here).
+bool linear_few_wanted(int64_t M, int64_t N, int64_t K, int in_type) { return M <= (in_type == GNN_F32 ? 32 : 8); }
 
 int launch_linear_few(const TcOperand& a, const TcOperand& b, int in_type, int64_t M, int64_t N, int64_t K,
                       const LinearEpilogue& ep, cudaStream_t stream, const char* what) {
@@ -276,7 +272,8 @@ int launch_linear_few(const TcOperand& a, const TcOperand& b, int in_type, int64
     launch(few_fma_kernel<8, 4>, ctas, cluster_for(ctas, (p.row_bytes + 511) / 512), p, stream);
   } else {
     const int64_t ctas = (N + 3) / 4;
-    launch(few_fma_kernel<4, 8>, ctas, cluster_for(ctas, (p.row_bytes + 511) / 512), p, stream);
+    const int groups = (int)((M + 7) / 8);
+    launch(few_fma_kernel<4, 8>, ctas, cluster_for(ctas * groups, (p.row_bytes + 511) / 512), p, stream, groups);
   }
   return check_launch(what);
 }

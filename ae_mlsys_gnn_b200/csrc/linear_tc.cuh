@@ -43,6 +43,18 @@ bool linear_few_wanted(int64_t M, int64_t N, int64_t K, int in_type);
 int launch_linear_few(const TcOperand& a, const TcOperand& b, int in_type, int64_t M, int64_t N, int64_t K,
                       const LinearEpilogue& ep, cudaStream_t stream, const char* what);
 
+// The same product for up to 128 rows of 16-bit or 8-bit operands (linear_narrow.cu), both K-major;
+// no workspace.
+bool linear_narrow_wanted(int64_t M, int64_t K, int in_type);
+int launch_linear_narrow(const TcOperand& a, const TcOperand& b, int in_type, int64_t M, int64_t N, int64_t K,
+                         const LinearEpilogue& ep, int* status, cudaStream_t stream, const char* what);
+
+// Longest chain of stages (of 128 bytes) that one accumulator takes.  The tensor cores cut off what
+// does not fit the running sum: sums of same-sign products come out low by about 2^-23 of their value
+// per MMA step, four steps a stage (measured: 1.1e-4 after 1,094 steps of fp16).  The limits keep
+// that below half a step of the result: 8e-4 in bf16 (2^-9), 1.1e-4 in fp16 (2^-12).
+inline int64_t max_chain(int in_type) { return in_type == GNN_F16 ? 256 : 2048; }
+
 // TMA reads an operand whose rows are a multiple of 16 bytes apart and 16-byte aligned.
 inline bool tma_operand_ok(const TcOperand& o, int elt) {
   return (reinterpret_cast<uintptr_t>(o.p) & 15) == 0 && o.ld * elt % 16 == 0;

@@ -94,8 +94,10 @@ def test_linear_c_refusals():
     assert fwd(it=F32, ot=F32, K=62, ldx=62, ldw=62, M=100) == -4
     assert fwd(it=F32, ot=F32, M=100) == -3  # no scratch
     need = ctypes.c_size_t(0)
-    assert lib.gnn_linear_fwd_workspace_bytes(64, 70, 9000, BF16, ctypes.byref(need)) == 0 and need.value > 0
-    assert fwd(M=64, N=70, K=9000, ldx=9000, ldw=9000) == -3
+    # few rows need no scratch, many rows of a long reduction do
+    assert lib.gnn_linear_fwd_workspace_bytes(64, 70, 9000, BF16, ctypes.byref(need)) == 0 and need.value == 0
+    assert lib.gnn_linear_fwd_workspace_bytes(300, 70, 9000, BF16, ctypes.byref(need)) == 0 and need.value > 0
+    assert fwd(M=300, N=70, K=9000, ldx=9000, ldw=9000) == -3
     assert lib.gnn_linear_fwd_workspace_bytes(64, 70, 9000, 5, ctypes.byref(need)) == -1
     act = lambda gy=ONE, z=ONE, a=4, ldz=8, ws=ONE, nb=1 << 20, gz=ONE, gb=ONE, dt=BF16: lib.gnn_linear_act_bwd(
         gy, z, a, 0.2, dt, 4, 8, gz, ldz, gb, ws, nb, None)
