@@ -8,6 +8,7 @@ pointers plus sizes.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 
 import torch
@@ -241,15 +242,42 @@ def call(name: str, *args) -> None:
     t.records.append((name, a, b))
 
 
+_functions: dict[str, "C._CFuncPtr"] = {}
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+else:
+    def _raw_stream(index: int) -> int:
+        return torch.cuda.current_stream(index).cuda_stream
+
+
 def launch(dev: torch.device, name: str, *args) -> None:
-    """``call`` on ``dev`` and its current stream, which is passed as the last argument.  The current
-    device is switched only when it is another one (small calls are bound by the host)."""
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    if dev.index == torch.cuda.current_device():
-        call(name, *args, stream)
-    else:
-        with torch.cuda.device(dev):
-            call(name, *args, stream)
+    """``call`` on ``dev`` and its current stream, which is passed as the last argument.  Small calls
+    are bound by the host, so the current device is switched only when it is another one."""
+    index = dev.index
+    if _timer is None and index == _current_device():
+        fn = _functions.get(name)
+        if fn is None:
+            fn = _functions[name] = getattr(lib(), name)
+        rc = fn(*args, _raw_stream(index))
+        if rc != 0:
+            check(rc, name)
+        return
+    with torch.cuda.device(dev):
+        call(name, *args, _raw_stream(index))
+
+
+@functools.lru_cache(maxsize=4096)
+def scratch_bytes(name: str, *sizes) -> int:
+    """``workspace_bytes`` of the entry points whose answer depends on the sizes alone, remembered."""
+    return workspace_bytes(name, *sizes)
+
+
+def scratch(name: str, dev: torch.device, *sizes):
+    """(buffer or None, bytes): scratch of one call, from torch's allocator, so that two captured
+    graphs, or two streams, never share it."""
+    nbytes = scratch_bytes(name, *sizes)
+    return (torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None), nbytes
 
 
 def workspace_bytes(name: str, *args) -> int:
@@ -285,26 +313,33 @@ def require(t: torch.Tensor, dtype: torch.dtype, name: str, ndim: int | None = N
     return t
 
 
-def rows_of(t: torch.Tensor, name: str, width: int | None = None, like: torch.Tensor | None = None) -> torch.Tensor:
+def rows_of(t: torch.Tensor, name: str, like: torch.Tensor | None = None) -> torch.Tensor:
     """Validation of a matrix of rows in one of the feed-forward types, with any number of leading
-    dimensions: CUDA device, type, last dimension; ``like``: same device, type and shape.  Rows
-    that are not laid out one after the other are copied."""
+    dimensions: CUDA device and type (``like``: the same as that tensor's).  Rows that are not laid out
+    one after the other are copied."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor (no CPU path exists)")
-    if t.dtype not in DTYPE_CODES:
+    if like is not None:
+        if t.dtype is not like.dtype:
+            raise TypeError(f"{name} must be {like.dtype}, got {t.dtype}")
+        if t.device != like.device:
+            raise ValueError(f"{name} is on {t.device}, expected {like.device}")
+    elif t.dtype not in DTYPE_CODES:
         raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
     if t.dim() < 1:
         raise ValueError(f"{name} must have at least 1 dim")
-    if width is not None and t.shape[-1] != width:
-        raise ValueError(f"{name} must have {width} columns, got shape {tuple(t.shape)}")
-    if like is not None:
-        if t.device != like.device:
-            raise ValueError(f"{name} is on {t.device}, expected {like.device}")
-        if t.dtype != like.dtype:
-            raise TypeError(f"{name} must be {like.dtype}, got {t.dtype}")
     return t if t.is_contiguous() else t.contiguous()
+
+
+def recorded(*tensors) -> bool:
+    """Whether autograd has to record a call on these tensors (None: absent)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 _workspaces: dict[tuple[int, int], torch.Tensor] = {}

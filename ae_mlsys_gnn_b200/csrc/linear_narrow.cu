@@ -209,10 +209,11 @@ int launch_instance(const CUtensorMap& mw, const CUtensorMap& mx, NarrowParams p
   constexpr int kStageBytes = kATile + BN * kStageK;
   auto kernel = linear_narrow_kernel<BN, FP8, T>;
   const int fixed = 1024 + kBarBytes;
-  p.stages = (232448 - 64 - fixed) / kStageBytes;
+  p.stages = (kSmemLimit - 64 - fixed) / kStageBytes;
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   const int smem = fixed + p.stages * kStageBytes;
-  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static SmemGrant grant;
+  grant.allow(kernel, kSmemLimit - 64);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((p.N + BM - 1) / BM * p.cluster));
   cfg.blockDim = dim3(kThreads);

@@ -44,7 +44,6 @@ constexpr int kMaxStages = 7;
 constexpr int kNumBars = 2 * kMaxStages + 4 + kEpiWarps;
 constexpr int kBarBytes = (8 * kNumBars + 16 + 127) / 128 * 128;
 constexpr int kUnitBytes = 32 * 128;                // 32 rows x 128 bytes of output
-constexpr int kSmemLimit = 232448;
 
 template <int BN, bool PAIR>
 struct Geom {
@@ -580,7 +579,8 @@ int launch_instance(const Maps& m, Params p, int grid, cudaStream_t stream) {
   p.stages = (kSmemLimit - 64 - fixed) / G::kStageBytes;
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   const int smem = fixed + p.stages * G::kStageBytes;
-  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static SmemGrant grant;
+  grant.allow(kernel, kSmemLimit - 64);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(kThreads);

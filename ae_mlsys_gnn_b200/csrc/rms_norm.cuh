@@ -1,7 +1,7 @@
 // Row layout shared by the root-mean-square norm kernels.
 //
-// A row of d elements belongs to a group of G threads (a power of two: 4..32 lanes of one warp,
-// or whole warps); thread t of the group owns the vectors t, t + G, t + 2G, ... (NV of them,
+// A row of d elements belongs to a group of G threads (4, 8, 16 or 32 lanes of one warp, or any
+// number of whole warps); thread t of the group owns the vectors t, t + G, t + 2G, ... (NV of them,
 // VEC elements each), holds them in registers from the load to the store, and the row is
 // therefore read once.  EPT = NV * VEC elements per thread.
 #pragma once
@@ -72,8 +72,9 @@ inline NormGeom norm_geom(int64_t d, int vec, int ept, int min_group) {
   g.vec = vec;
   g.ept = ept;
   int need = (int)((d + ept - 1) / ept), group = min_group;
-  while (group < need) group *= 2;
-  g.group = group;
+  while (group < need && group < 32) group *= 2;
+  g.group = need > 32 ? (need + 31) / 32 * 32 : group;
+  group = g.group;
   g.threads = group > 32 ? group : 128;
   g.rows = g.threads / group;
   return g;

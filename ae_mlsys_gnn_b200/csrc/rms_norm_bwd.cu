@@ -36,7 +36,7 @@ struct RowParts {
 };
 
 template <class T, int VEC, int NV, int MAXT>
-__global__ void __launch_bounds__(MAXT) rms_norm_bwd_kernel(const BwdParams p) {
+__global__ void __launch_bounds__(MAXT, sizeof(T) * VEC * NV <= 16 ? 2 : 1) rms_norm_bwd_kernel(const BwdParams p) {
   __shared__ float s_sum[2][32];
   extern __shared__ float s_gw[];  // [d], groups within one warp only
   using P = Pack<T, VEC>;
@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(MAXT) rms_norm_bwd_kernel(const BwdParams p) {
   // (32 elements a thread) the registers do not suffice, and more bytes are in flight anyway.
   constexpr bool kAhead = NV * VEC <= 16, kKeepWeight = NV * VEC <= 8;
   const int G = p.group;
-  const int t = threadIdx.x & (G - 1), local = threadIdx.x / G;
+  const int local = threadIdx.x / G, t = threadIdx.x - local * G;
   const int rows = blockDim.x / G;
   const int nvec = p.d / VEC;
   const T* const gy = static_cast<const T*>(p.gy);
@@ -176,8 +176,8 @@ __global__ void __launch_bounds__(1024) weight_grad_kernel(const float* __restri
 NormGeom pick_bwd(int64_t d, int vec) {
   NormGeom g = norm_geom(d, vec, norm_ept(d), 4);
   if (g.group <= 128) {  // several rows side by side
-    g.threads = 256;
-    g.rows = g.threads / g.group;
+    g.rows = 256 / g.group;
+    g.threads = g.rows * g.group;
   }
   return g;
 }

@@ -32,13 +32,13 @@ struct FwdParams {
 };
 
 template <class T, int VEC, int NV, bool FP8, int MAXT>
-__global__ void __launch_bounds__(MAXT) rms_norm_kernel(const FwdParams p) {
+__global__ void __launch_bounds__(MAXT, sizeof(T) * VEC * NV <= 16 ? 4 : 1) rms_norm_kernel(const FwdParams p) {
   __shared__ float s_sum[32];
   __shared__ int s_max[32];
   extern __shared__ int s_block_max[];  // [rows of this CTA][n_blocks], FP8 with block scales
   const int G = p.group;
-  const int t = threadIdx.x & (G - 1);
   const int local = threadIdx.x / G;
+  const int t = threadIdx.x - local * G;
   const int64_t row = (int64_t)blockIdx.x * (blockDim.x / G) + local;
   const bool live = row < p.n;
   using P = Pack<T, VEC>;
@@ -150,10 +150,10 @@ __global__ void __launch_bounds__(MAXT) rms_norm_kernel(const FwdParams p) {
     for (int i = 0; i < NV; ++i) {
       const int col = (t + G * i) * VEC;
       if (col < p.d) {
-        const float s = p.block ? scale_of(bm[col / 128]) : row_scale;
+        const float inv = 1.f / (p.block ? scale_of(bm[col / 128]) : row_scale);
         Pack<uint8_t, VEC> o;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) o.v[j] = __nv_cvt_float_to_fp8(v[i][j] / s, __NV_SATFINITE, __NV_E4M3);
+        for (int j = 0; j < VEC; ++j) o.v[j] = __nv_cvt_float_to_fp8(v[i][j] * inv, __NV_SATFINITE, __NV_E4M3);
         store_pack(reinterpret_cast<Pack<uint8_t, VEC>*>(p.q + row * p.d + col), o);
       }
     }

@@ -2,6 +2,7 @@
 // tensor maps of their operands.
 #pragma once
 #include <cuda.h>
+#include <atomic>
 #include "common.cuh"
 #include "linear_tc.cuh"
 
@@ -142,6 +143,20 @@ __device__ __forceinline__ void umma_commit(uint32_t bar) {
   else
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
+
+// Lets one kernel use `bytes` of shared memory, once per device (a static object of its launcher).
+struct SmemGrant {
+  std::atomic<uint64_t> done{0};
+  template <class Kernel>
+  void allow(Kernel kernel, int bytes) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess) done.fetch_or(bit);
+  }
+};
+constexpr int kSmemLimit = 232448;  // shared memory of a CTA, static included
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,

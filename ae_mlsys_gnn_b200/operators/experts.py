@@ -49,10 +49,9 @@ def expert_sort(ids, n_experts: int) -> ExpertOrder:
     dev = ids.device
     slots = torch.empty(ids.shape, dtype=I32, device=dev)
     offsets = torch.empty(n_experts + 1, dtype=I32, device=dev)
-    nbytes = capi.workspace_bytes("gnn_expert_sort_workspace_bytes", ids.numel(), n_experts)
-    # scratch of this call alone: two captured graphs, or two streams, never share it
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    capi.launch(dev, "gnn_expert_sort", ids.data_ptr(), int(ids.dtype == torch.int64), ids.numel(), n_experts,
+    pairs = ids.numel()
+    ws, nbytes = capi.scratch("gnn_expert_sort_workspace_bytes", dev, pairs, n_experts)
+    capi.launch(dev, "gnn_expert_sort", ids.data_ptr(), int(ids.dtype is torch.int64), pairs, n_experts,
                 offsets.data_ptr(), slots.data_ptr(), capi.ptr(ws), nbytes)
     return ExpertOrder(offsets, slots, n_experts)
 
@@ -125,7 +124,7 @@ def expert_dispatch(x, order: ExpertOrder):
     _check_order(order, x.device)
     if x.dim() != 2 or x.shape[0] != order.tokens:
         raise ValueError(f"x must be ({order.tokens}, D), got {tuple(x.shape)}")
-    if x.requires_grad and torch.is_grad_enabled():
+    if capi.recorded(x):
         return _Dispatch.apply(x, order)
     return _dispatch(x, order)
 
@@ -144,6 +143,6 @@ def expert_combine(rows, weights, order: ExpertOrder):
         raise ValueError(f"weights is on {weights.device}, expected {rows.device}")
     if weights.shape != order.slots.shape:
         raise ValueError(f"weights must be {tuple(order.slots.shape)}, got {tuple(weights.shape)}")
-    if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
+    if capi.recorded(rows, weights):
         return _Combine.apply(rows, weights, order)
     return _combine(rows, weights, order)

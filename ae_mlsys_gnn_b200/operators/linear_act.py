@@ -26,6 +26,7 @@ ACTIVATIONS = {None: 0, "relu": 1, "leaky_relu": 2, "elu": 3, "gelu": 4, "silu":
 
 
 def _status(dev):
+    """The device's status word; it has to outlive every graph, so it is not made while one is captured."""
     t = dense._status.get(dev.index)
     if t is None:
         if torch.cuda.is_current_stream_capturing():
@@ -34,21 +35,15 @@ def _status(dev):
     return t
 
 
-def _scratch(name, dev, *sizes):
-    """Scratch of one call: two captured graphs, or two streams, never share it."""
-    nbytes = capi.workspace_bytes(name, *sizes)
-    return (torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None), nbytes
-
-
 def _operand(t):
     """(tensor, row pitch in elements) of a contiguous matrix as the product kernels read it: rows a
     multiple of 16 bytes apart that start on a 16-byte boundary; others are copied to such a pitch (for
     fp32 the columns behind the last are zeros, which the reduction runs over)."""
     k = t.shape[1]
     per = 16 // t.element_size()
-    ld = -(-k // per) * per
-    if ld == k:
+    if k % per == 0:
         return (t if t.data_ptr() % 16 == 0 else t.clone()), k
+    ld = -(-k // per) * per
     buf = torch.empty((t.shape[0], ld), dtype=t.dtype, device=t.device)
     buf[:, :k] = t
     if t.dtype == torch.float32:
@@ -67,10 +62,11 @@ def _forward(x, xs, weight, ws, bias, act, residual, slope, out_dtype, want_z):
     if code == 0:
         K = ldx  # zero columns behind the last
     if M and N:
-        scratch, nbytes = _scratch("gnn_linear_fwd_workspace_bytes", dev, M, N, K, code)
-        capi.launch(dev, "gnn_linear_fwd", x.data_ptr(), ldx, weight.data_ptr(), ldw, code, capi.ptr(xs), capi.ptr(ws),
-                    capi.ptr(bias), act, slope, capi.ptr(residual), y.data_ptr(), capi.ptr(z),
-                    capi.DTYPE_CODES[out_dtype], M, N, K, capi.ptr(scratch), nbytes, _status(dev).data_ptr())
+        scratch, nbytes = capi.scratch("gnn_linear_fwd_workspace_bytes", dev, M, N, K, code)
+        ptr = capi.ptr
+        capi.launch(dev, "gnn_linear_fwd", x.data_ptr(), ldx, weight.data_ptr(), ldw, code, ptr(xs), ptr(ws), ptr(bias), act,
+                    slope, ptr(residual), y.data_ptr(), ptr(z), capi.DTYPE_CODES[out_dtype], M, N, K, ptr(scratch), nbytes,
+                    _status(dev).data_ptr())
     return y, z
 
 
@@ -106,7 +102,7 @@ class _LinearAct(torch.autograd.Function):
         if need_b:
             gb = torch.empty(N, dtype=dt, device=dev)
         if own_gz or need_b:
-            scratch, nbytes = _scratch("gnn_linear_act_bwd_workspace_bytes", dev, M, N, ldz) if need_b else (None, 0)
+            scratch, nbytes = capi.scratch("gnn_linear_act_bwd_workspace_bytes", dev, M, N, ldz) if need_b else (None, 0)
             capi.launch(dev, "gnn_linear_act_bwd", gy.data_ptr(), capi.ptr(z), act, slope, code, M, N,
                         gz.data_ptr() if own_gz else None, ldz, capi.ptr(gb), capi.ptr(scratch), nbytes)
         if need_x:
@@ -119,7 +115,7 @@ class _LinearAct(torch.autograd.Function):
                         wr = torch.nn.functional.pad(w, (0, 0, 0, n - N))
                     if k != K:
                         out = torch.empty((M, k), dtype=dt, device=dev)
-                scratch, nbytes = _scratch("gnn_linear_dgrad_workspace_bytes", dev, M, n, k, code)
+                scratch, nbytes = capi.scratch("gnn_linear_dgrad_workspace_bytes", dev, M, n, k, code)
                 capi.launch(dev, "gnn_linear_dgrad", gz.data_ptr(), ldz, wr.data_ptr(), wr.shape[1], code, out.data_ptr(),
                             M, n, k, capi.ptr(scratch), nbytes, _status(dev).data_ptr())
                 if out is not gx:
@@ -131,7 +127,7 @@ class _LinearAct(torch.autograd.Function):
                 n, k = ldz, x.shape[1]
                 if n != N or k != K:
                     out = torch.empty((n, k), dtype=dt, device=dev)
-            scratch, nbytes = _scratch("gnn_linear_wgrad_workspace_bytes", dev, M, n, k, code)
+            scratch, nbytes = capi.scratch("gnn_linear_wgrad_workspace_bytes", dev, M, n, k, code)
             capi.launch(dev, "gnn_linear_wgrad", gz.data_ptr(), ldz, x.data_ptr(), x.shape[1], code, out.data_ptr(), M, n,
                         k, capi.ptr(scratch), nbytes, _status(dev).data_ptr())
             if out is not gw:
@@ -160,11 +156,11 @@ def linear_act(x, weight, bias=None, activation=None, residual=None, negative_sl
     one type: float32, bfloat16 or float16.  ``activation``: None, "relu", "leaky_relu" (with
     ``negative_slope``), "elu", "gelu" (the erf form) or "silu".  Differentiable in all four tensors."""
     x = capi.rows_of(x, "x")
-    weight = capi.rows_of(weight, "weight", None, x)
+    weight = capi.rows_of(weight, "weight", x)
     if weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
         raise ValueError(f"weight must be (N, {x.shape[-1]}), got {tuple(weight.shape)}")
-    if x.shape[-1] < 1:
-        raise ValueError("x must have at least one column")
+    if x.shape[-1] < 1 or weight.shape[0] < 1:
+        raise ValueError("x must have at least one column and weight at least one row")
     lead, N = x.shape[:-1], weight.shape[0]
     _check_epilogue(lead, N, x.dtype, x.device, bias, activation, residual)
     act, slope = ACTIVATIONS[activation], float(negative_slope)
@@ -175,8 +171,7 @@ def linear_act(x, weight, bias=None, activation=None, residual=None, negative_sl
             residual = residual.view(-1, N)
     if bias is not None:
         bias = bias.contiguous()
-    if torch.is_grad_enabled() and (x2.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
+    if capi.recorded(x2, weight, bias, residual):
         y = _LinearAct.apply(x2, weight, bias, residual, act, slope)
     else:
         y, _ = _forward((*_operand(x2), x2.shape[1]), None, _operand(weight), None, bias, act, residual, slope, x.dtype,
@@ -212,19 +207,24 @@ def linear_act_fp8(x8, x_scale, weight8, weight_scale, bias=None, activation=Non
     dev = x8.device
     if weight8.device != dev:
         raise ValueError(f"weight8 is on {weight8.device}, expected {dev}")
-    if x8.dim() < 1 or weight8.dim() != 2 or weight8.shape[1] != x8.shape[-1] or x8.shape[-1] < 1:
+    if x8.dim() < 1 or weight8.dim() != 2 or weight8.shape[1] != x8.shape[-1] or weight8.numel() < 1:
         raise ValueError(f"x8 must be (..., K) and weight8 (N, K), got {tuple(x8.shape)} and {tuple(weight8.shape)}")
     if out_dtype not in capi.DTYPE_CODES:
         raise TypeError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
     lead, N, K = x8.shape[:-1], weight8.shape[0], x8.shape[-1]
     _check_epilogue(lead, N, out_dtype, dev, bias, activation, residual)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x_scale, weight_scale, bias, residual)):
-        raise RuntimeError("linear_act_fp8 has no gradient: call it under torch.no_grad()")
-    x2 = x8.contiguous().view(-1, K)
+    x2 = x8.contiguous()
+    if x2.dim() != 2:
+        x2 = x2.view(-1, K)
     xs = _scale_of(x_scale, "x_scale", x2.shape[0], dev)
     ws = _scale_of(weight_scale, "weight_scale", N, dev)
+    if capi.recorded(xs, ws, bias, residual):
+        raise RuntimeError("linear_act_fp8 has no gradient: call it under torch.no_grad()")
+    if bias is not None:
+        bias = bias.contiguous()
+    if residual is not None:
+        residual = residual.contiguous()
     xo, ldx = _operand(x2)
-    y, _ = _forward((xo, ldx, K), xs, _operand(weight8.contiguous()), ws, None if bias is None else bias.contiguous(),
-                    ACTIVATIONS[activation], None if residual is None else residual.contiguous().view(-1, N),
+    y, _ = _forward((xo, ldx, K), xs, _operand(weight8.contiguous()), ws, bias, ACTIVATIONS[activation], residual,
                     float(negative_slope), out_dtype, False)
     return y if x8.dim() == 2 else y.view(*lead, N)

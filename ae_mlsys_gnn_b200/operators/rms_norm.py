@@ -22,30 +22,30 @@ def _check(x, weight, residual):
     d = x.shape[-1]
     if d < 1:
         raise ValueError("x must have at least one column")
-    if not isinstance(weight, torch.Tensor) or weight.dim() != 1:
-        raise ValueError("weight must be a vector of x's width")
-    if weight.dtype == torch.float32 and x.dtype != torch.float32:
-        weight = capi.require(weight.contiguous(), torch.float32, "weight", 1, x.device)
+    if isinstance(weight, torch.Tensor) and weight.dtype is torch.float32:
+        weight = capi.rows_of(weight, "weight")
+        if weight.device != x.device:
+            raise ValueError(f"weight is on {weight.device}, expected {x.device}")
     else:
-        weight = capi.rows_of(weight, "weight", None, x)
-    if weight.shape[0] != d:
-        raise ValueError(f"weight must have {d} elements, got {weight.shape[0]}")
+        weight = capi.rows_of(weight, "weight", x)
+    if weight.dim() != 1 or weight.shape[0] != d:
+        raise ValueError(f"weight must be a vector of {d} elements, got shape {tuple(weight.shape)}")
     if residual is not None:
-        residual = capi.rows_of(residual, "residual", None, x)
+        residual = capi.rows_of(residual, "residual", x)
         if residual.shape != x.shape:
             raise ValueError(f"residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
-    return x, weight, residual
+    return x, weight, residual, d
 
 
-def _forward(x, weight, residual, eps, with_rstd):
-    d = x.shape[-1]
-    n = x.numel() // d
+def _forward(x, weight, residual, eps, d, with_rstd):
+    dev, n = x.device, x.numel() // d
     y = torch.empty_like(x)
     h = torch.empty_like(x) if residual is not None else None
-    rstd = torch.empty(n, dtype=torch.float32, device=x.device) if with_rstd else None
-    capi.launch(x.device, "gnn_rms_norm_fwd", x.data_ptr(), capi.ptr(residual), weight.data_ptr(),
-                capi.DTYPE_CODES[x.dtype], capi.DTYPE_CODES[weight.dtype], n, d, eps, y.data_ptr(), capi.ptr(h),
-                capi.ptr(rstd))
+    rstd = torch.empty(n, dtype=torch.float32, device=dev) if with_rstd else None
+    code = capi.DTYPE_CODES
+    capi.launch(dev, "gnn_rms_norm_fwd", x.data_ptr(), None if residual is None else residual.data_ptr(),
+                weight.data_ptr(), code[x.dtype], code[weight.dtype], n, d, eps, y.data_ptr(),
+                None if h is None else h.data_ptr(), None if rstd is None else rstd.data_ptr())
     return y, h, rstd
 
 
@@ -53,7 +53,7 @@ class _AddRmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
         ctx.set_materialize_grads(False)
-        y, h, rstd = _forward(x, weight, residual, eps, True)
+        y, h, rstd = _forward(x, weight, residual, eps, x.shape[-1], True)
         ctx.save_for_backward(x if h is None else h, weight, rstd)
         ctx.has_residual = h is not None
         return (y, h) if h is not None else y
@@ -73,9 +73,7 @@ class _AddRmsNorm(torch.autograd.Function):
         nbytes = 0
         if ctx.needs_input_grad[1]:
             gw = torch.empty_like(weight)
-            nbytes = capi.workspace_bytes("gnn_rms_norm_bwd_workspace_bytes", n, d)
-            # scratch of this call alone: two captured graphs, or two streams, never share it
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=h.device)
+            ws, nbytes = capi.scratch("gnn_rms_norm_bwd_workspace_bytes", h.device, n, d)
         capi.launch(h.device, "gnn_rms_norm_bwd", gy.data_ptr(), capi.ptr(gh), h.data_ptr(), weight.data_ptr(),
                     rstd.data_ptr(), capi.DTYPE_CODES[h.dtype], capi.DTYPE_CODES[weight.dtype], n, d, gx.data_ptr(),
                     capi.ptr(gw), capi.ptr(ws), nbytes)
@@ -85,12 +83,11 @@ class _AddRmsNorm(torch.autograd.Function):
 def add_rms_norm(x, weight, residual=None, eps: float = 1e-6):
     """(y, h) for x (..., D), weight (D,) of x's type or float32, residual of x's shape or None
     (then h is x itself).  Differentiable in x, weight and residual."""
-    x, weight, residual = _check(x, weight, residual)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
-                                    or (residual is not None and residual.requires_grad)):
+    x, weight, residual, d = _check(x, weight, residual)
+    if capi.recorded(x, weight, residual):
         out = _AddRmsNorm.apply(x, weight, residual, float(eps))
         return out if residual is not None else (out, x)
-    y, h, _ = _forward(x, weight, residual, eps, False)
+    y, h, _ = _forward(x, weight, residual, eps, d, False)
     return y, (x if h is None else h)
 
 
@@ -99,18 +96,17 @@ def add_rms_norm_fp8(x, weight, residual=None, eps: float = 1e-6, block: int = 0
     y ~ q * scale, scale = max(max|y| / 448, 2^-126) over a row (``block`` 0, scale (..., 1)) or over
     every 128 columns (``block`` 128, scale (..., ceil(D / 128))).  For inference: inputs that
     require a gradient are refused while gradients are recorded."""
-    x, weight, residual = _check(x, weight, residual)
+    x, weight, residual, d = _check(x, weight, residual)
     if block not in (0, 128):
         raise ValueError("block must be 0 (one scale a row) or 128")
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
-                                    or (residual is not None and residual.requires_grad)):
+    if capi.recorded(x, weight, residual):
         raise RuntimeError("add_rms_norm_fp8 has no gradient: call it under torch.no_grad()")
-    d = x.shape[-1]
-    n = x.numel() // d
-    q = torch.empty(x.shape, dtype=FP8, device=x.device)
-    scale = torch.empty((*x.shape[:-1], -(-d // block) if block else 1), dtype=torch.float32, device=x.device)
+    dev, n = x.device, x.numel() // d
+    q = torch.empty_like(x, dtype=FP8)
+    scale = torch.empty((*x.shape[:-1], -(-d // block) if block else 1), dtype=torch.float32, device=dev)
     h = torch.empty_like(x) if residual is not None else None
-    capi.launch(x.device, "gnn_rms_norm_fp8", x.data_ptr(), capi.ptr(residual), weight.data_ptr(),
-                capi.DTYPE_CODES[x.dtype], capi.DTYPE_CODES[weight.dtype], n, d, eps, block, q.data_ptr(),
-                scale.data_ptr(), capi.ptr(h))
+    code = capi.DTYPE_CODES
+    capi.launch(dev, "gnn_rms_norm_fp8", x.data_ptr(), None if residual is None else residual.data_ptr(),
+                weight.data_ptr(), code[x.dtype], code[weight.dtype], n, d, eps, block, q.data_ptr(), scale.data_ptr(),
+                None if h is None else h.data_ptr())
     return q, scale, (x if h is None else h)
