@@ -60,73 +60,86 @@ __global__ void __launch_bounds__(MAXT, sizeof(T) * VEC * NV <= 16 ? 2 : 1) rms_
       if (t + G * i < nvec) load_weight<T, VEC>(p.weight, p.w_f32, (int64_t)(t + G * i) * VEC, wk[i]);
   }
 
-  auto request = [&](int64_t row, RowParts<T, VEC, NV>& q) {
+  const int64_t step = (int64_t)gridDim.x * rows;
+  int64_t row = (int64_t)blockIdx.x * rows + local;  // of the parts requested next
+  int64_t at = row * p.d + (int64_t)t * VEC;
+  const int64_t stride = step * p.d;
+  auto request = [&](RowParts<T, VEC, NV>& q) {
     if (row >= p.n) return;
     q.rstd = p.rstd[row];
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (t + G * i < nvec) {
-        const int64_t at = row * p.d + (int64_t)(t + G * i) * VEC;
-        q.gy[i] = load_pack(reinterpret_cast<const P*>(gy + at));
-        q.h[i] = load_pack(reinterpret_cast<const P*>(h + at));
-        if (gh) q.gh[i] = load_pack(reinterpret_cast<const P*>(gh + at));
+        q.gy[i] = load_pack(reinterpret_cast<const P*>(gy + at) + G * i);
+        q.h[i] = load_pack(reinterpret_cast<const P*>(h + at) + G * i);
+        if (gh) q.gh[i] = load_pack(reinterpret_cast<const P*>(gh + at) + G * i);
       }
   };
-  // u = grad_y * weight, x = xhat of vector i
-  auto unpack = [&](const RowParts<T, VEC, NV>& q, int i, float (&g)[VEC], float (&u)[VEC], float (&x)[VEC]) {
-    float w[VEC];
-    q.gy[i].widen(g);
-    q.h[i].widen(x);
-    if constexpr (!kKeepWeight) load_weight<T, VEC>(p.weight, p.w_f32, (int64_t)(t + G * i) * VEC, w);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      x[j] *= q.rstd;
-      u[j] = g[j] * (kKeepWeight ? wk[kKeepWeight ? i : 0][j] : w[j]);
-    }
-  };
 
+  // With s = rstd * grad_y * weight the products of a row are
+  //   dot = sum(s * h) = sum(u * xhat),  grad_w += (rstd * grad_y) * h,
+  //   grad_x = s - (rstd^2 * dot / d) * h + grad_h
+  // and s stays in registers between the two halves (wide shares form it again).
   RowParts<T, VEC, NV> cur, next;
-  const int64_t step = (int64_t)gridDim.x * rows;
-  int64_t row = (int64_t)blockIdx.x * rows + local;
-  request(row, kAhead ? next : cur);
+  if constexpr (kAhead) request(next);
   int turn = 0;
+  const float inv_d = 1.f / (float)p.d;
   // every thread of the CTA makes the same number of turns: the sums below are collective
-  for (int64_t first = (int64_t)blockIdx.x * rows; first < p.n; first += step, row += step, turn ^= 1) {
+  for (int64_t first = (int64_t)blockIdx.x * rows; first < p.n; first += step, turn ^= 1) {
     const bool live = row < p.n;
+    T* const gx = static_cast<T*>(p.gx) + at;
     if constexpr (kAhead) {
       cur = next;
-      request(row + step, next);
-    } else if (first != (int64_t)blockIdx.x * rows) {
-      request(row, cur);
+      row += step;
+      at += stride;
+      request(next);
+    } else {
+      request(cur);
+      row += step;
+      at += stride;
     }
+    float s[kAhead ? NV : 1][VEC];
+    auto scaled = [&](int i, float (&g)[VEC], float (&out)[VEC]) {  // g = rstd * grad_y, out = s
+      cur.gy[i].widen(g);
+      float w[VEC];
+      if constexpr (!kKeepWeight) load_weight<T, VEC>(p.weight, p.w_f32, (int64_t)(t + G * i) * VEC, w);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        g[j] *= cur.rstd;
+        out[j] = g[j] * (kKeepWeight ? wk[kKeepWeight ? i : 0][j] : w[j]);
+      }
+    };
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (live && t + G * i < nvec) {
         float g[VEC], u[VEC], x[VEC];
-        unpack(cur, i, g, u, x);
+        scaled(i, g, u);
+        cur.h[i].widen(x);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           gw[i][j] = fmaf(g[j], x[j], gw[i][j]);
           dot = fmaf(u[j], x[j], dot);
+          if constexpr (kAhead) s[i][j] = u[j];
         }
       }
-    const float mean = group_sum(dot, G, s_sum[turn]) / (float)p.d;
+    const float c = -cur.rstd * (cur.rstd * (group_sum(dot, G, s_sum[turn]) * inv_d));
     if (live) {
-      T* const gx = static_cast<T*>(p.gx) + row * p.d;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (t + G * i < nvec) {
           float g[VEC], u[VEC], x[VEC];
-          unpack(cur, i, g, u, x);
+          if constexpr (!kAhead) scaled(i, g, u);
+          cur.h[i].widen(x);
 #pragma unroll
           for (int j = 0; j < VEC; ++j) {
-            u[j] = cur.rstd * (u[j] - x[j] * mean);
-            if (gh) u[j] += to_f32(cur.gh[i].v[j]);
+            float v = kAhead ? s[kAhead ? i : 0][j] : u[j];
+            if (gh) v += to_f32(cur.gh[i].v[j]);
+            u[j] = fmaf(c, x[j], v);
           }
           P o;
           o.round(u);
-          store_pack(reinterpret_cast<P*>(gx) + t + G * i, o);
+          store_pack(reinterpret_cast<P*>(gx) + G * i, o);
         }
     }
   }
