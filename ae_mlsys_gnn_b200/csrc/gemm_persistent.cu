@@ -533,18 +533,30 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_
               }
             }
             __syncwarp();  // the block is rewritten by the next chunk
+          } else if (FINISH && last) {
+            // rows that are not whole 16-byte units: through the staging block as above, then a row at a
+            // time with neighbouring columns on neighbouring lanes
+            float4* const stg = epi_stage + (lg + 4 * part) * 256;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              stg[lane * 8 + (j ^ (lane & 7))] =
+                  make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]),
+                              __uint_as_float(r[4 * j + 3]));
+            __syncwarp();
+            const float* const flat = reinterpret_cast<const float*>(stg);
+            const int top = t.m0 + lg * 32;
+            if (col0 + lane < p.N) {
+#pragma unroll 4
+              for (int rr = 0; rr < 32; ++rr)
+                if (top + rr < p.M) {
+                  const int64_t at = (int64_t)(top + rr) * p.ldc + col0 + lane;
+                  Cout[at] = finish_one(p.fin, at, col0 + lane, flat[(rr * 8 + ((lane >> 2) ^ (rr & 7))) * 4 + (lane & 3)]);
+                }
+            }
+            __syncwarp();  // the block is rewritten by the next chunk
           } else if (last && row < p.M) {
             float* crow = Cout + (size_t)row * p.ldc + col0;
             const int ncols = min(32, p.N - col0);
-            if constexpr (FINISH) {
-              // one element at a time, for rows that are not whole 16-byte units
-              float* const mine = reinterpret_cast<float*>(epi_stage + (lg + 4 * part) * 256) + lane;
-#pragma unroll
-              for (int j = 0; j < 32; ++j) mine[j * 32] = __uint_as_float(r[j]);
-#pragma unroll 1
-              for (int j = 0; j < ncols; ++j)
-                crow[j] = finish_one(p.fin, (int64_t)row * p.ldc + col0 + j, col0 + j, mine[j * 32]);
-            } else
             if (ncols == 32 && ((uintptr_t)crow & 15) == 0) {
 #pragma unroll
               for (int j = 0; j < 32; j += 4)

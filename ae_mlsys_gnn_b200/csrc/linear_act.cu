@@ -8,8 +8,8 @@
 // 16-bit and 8-bit products run on linear_tc.cu, or for few rows on linear_few.cu and
 // linear_narrow.cu; fp32 ones on the error-compensated 3xTF32 kernel with the same epilogue.  The
 // tensor cores truncate when they add, so the fp32 kernel moves its sums to registers after every
-// kChain32 blocks of 32, i.e. 24 steps (relative error of random products of any length 5.7e-7;
-// 1.0e-6 with twice the chain).
+// kChain32 blocks of 32.  Relative error (2-norm, random operands) and time of 232965 x 604 -> 256 by
+// blocks in a chain: 2: 5.6e-7, 554 us; 3: 7.8e-7, 505 us; 4: 1.0e-6, 470 us.
 #include <stdio.h>
 #include <type_traits>
 #include "activation.cuh"
@@ -21,7 +21,7 @@
 namespace gnn {
 namespace {
 
-constexpr int kChain32 = 2;
+constexpr int kChain32 = 3, kChain32Long = 2;  // Long: the weights' gradient, whose reduction is the rows
 constexpr int kGroupCols = 8;  // columns a thread owns in the elementwise gradient
 
 int fail(int code, const char* what, const char* why) {
@@ -37,7 +37,7 @@ struct ActBwdParams {
   void* gz;         // nullptr: not wanted
   float* partial;   // [gridDim.y][N] column sums, nullptr: not wanted
   int64_t M, rows_per_cta;
-  int N, ldz, groups;  // ldz: elements from one row of gz to the next; groups: threads across columns (2^k <= 32)
+  int N, ldz, groups;  // ldz: elements from one row of gz to the next; groups: threads across columns (2^k <= 256)
   int act;
   float slope;
   int vec_ok;
@@ -46,7 +46,7 @@ struct ActBwdParams {
 // A CTA walks `rows_per_cta` rows of groups * 8 columns; a thread keeps its columns' sums in
 // registers.  HBM-bound: grad_y and z read, gz written once.
 template <class T>
-__global__ void __launch_bounds__(256) act_bwd_kernel(const ActBwdParams p) {
+__global__ void __launch_bounds__(256, 4) act_bwd_kernel(const ActBwdParams p) {
   __shared__ float s_sum[256][kGroupCols + 1];
   constexpr int V = 16 / (int)sizeof(T);
   const int g = threadIdx.x & (p.groups - 1), strand = threadIdx.x / p.groups, strands = blockDim.x / p.groups;
@@ -58,49 +58,63 @@ __global__ void __launch_bounds__(256) act_bwd_kernel(const ActBwdParams p) {
   const T* const gy = static_cast<const T*>(p.gy);
   const T* const z = static_cast<const T*>(p.z);
   T* const gz = static_cast<T*>(p.gz);
-  if (col < p.ldz) {
-#pragma unroll 2
+  if (p.vec_ok && col < p.N) {
+    // the loads of kRows rows are issued together, without branches between them (the compiler would
+    // neither move a load across the stores, which could alias, nor out of a condition it shares with
+    // its use); rows behind the last are read again and not counted
+    constexpr int kRows = sizeof(T) == 2 ? 2 : 1, Q = kGroupCols / V;  // twice as many spill at 64 registers
+    for (int64_t row0 = lo + strand; row0 < hi; row0 += strands * kRows) {
+      Pack<T, V> q[kRows][Q], r[kRows][Q];
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        const int64_t at = min(row0 + (int64_t)k * strands, hi - 1) * p.N + col;
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+          q[k][i] = load_pack(reinterpret_cast<const Pack<T, V>*>(gy + at) + i);
+          if (z) r[k][i] = load_pack(reinterpret_cast<const Pack<T, V>*>(z + at) + i);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        const int64_t row = row0 + (int64_t)k * strands;
+        if (row < hi) {
+          float v[kGroupCols], a[kGroupCols];
+#pragma unroll
+          for (int j = 0; j < kGroupCols; ++j) {
+            v[j] = to_f32(q[k][j / V].v[j % V]);
+            if (z) a[j] = to_f32(r[k][j / V].v[j % V]);
+          }
+          if (z) apply_act_slope<sizeof(T) == 4>(v, a, p.act, p.slope);
+#pragma unroll
+          for (int j = 0; j < kGroupCols; ++j) sum[j] += v[j];
+          if (gz) {
+#pragma unroll
+            for (int i = 0; i < Q; ++i) {
+              Pack<T, V> o;
+#pragma unroll
+              for (int j = 0; j < V; ++j) o.v[j] = from_f32<T>(v[i * V + j]);
+              store_pack(reinterpret_cast<Pack<T, V>*>(gz + row * p.ldz + col) + i, o);
+            }
+          }
+        }
+      }
+    }
+  } else if (!p.vec_ok && col < p.ldz) {
+#pragma unroll 1
     for (int64_t row = lo + strand; row < hi; row += strands) {
       const int64_t at = row * p.N + col;
       float v[kGroupCols], a[kGroupCols];
-      if (p.vec_ok) {
 #pragma unroll
-        for (int i = 0; i < kGroupCols; i += V) {
-          const Pack<T, V> q = load_pack(reinterpret_cast<const Pack<T, V>*>(gy + at + i));
-          Pack<T, V> r;
-          if (z) r = load_pack(reinterpret_cast<const Pack<T, V>*>(z + at + i));
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            v[i + j] = to_f32(q.v[j]);
-            if (z) a[i + j] = to_f32(r.v[j]);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < kGroupCols; ++j) {
-          const bool ok = col + j < p.N;
-          v[j] = ok ? to_f32(gy[at + j]) : 0.f;
-          a[j] = ok && z ? to_f32(z[at + j]) : 0.f;
-        }
+      for (int j = 0; j < kGroupCols; ++j) {
+        const bool ok = col + j < p.N;
+        v[j] = ok ? to_f32(gy[at + j]) : 0.f;
+        a[j] = ok && z ? to_f32(z[at + j]) : 0.f;
       }
       if (z) apply_act_slope<sizeof(T) == 4>(v, a, p.act, p.slope);
 #pragma unroll
-      for (int j = 0; j < kGroupCols; ++j) sum[j] += v[j];
-      if (gz) {
-        T* const o = gz + row * p.ldz + col;
-        if (p.vec_ok) {
-#pragma unroll
-          for (int i = 0; i < kGroupCols; i += V) {
-            Pack<T, V> q;
-#pragma unroll
-            for (int j = 0; j < V; ++j) q.v[j] = from_f32<T>(v[i + j]);
-            store_pack(reinterpret_cast<Pack<T, V>*>(o + i), q);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < kGroupCols; ++j)
-            if (col + j < p.ldz) o[j] = from_f32<T>(v[j]);  // the columns behind N are zeros
-        }
+      for (int j = 0; j < kGroupCols; ++j) {
+        sum[j] += v[j];
+        if (gz && col + j < p.ldz) gz[row * p.ldz + col + j] = from_f32<T>(v[j]);  // the columns behind N are zeros
       }
     }
   }
@@ -141,16 +155,34 @@ ActBwdGrid act_bwd_grid(int64_t M, int64_t ldz) {
   ActBwdGrid g;
   const int64_t need = (ldz + kGroupCols - 1) / kGroupCols;
   g.groups = 1;
-  while (g.groups < 32 && g.groups < need) g.groups *= 2;
+  while (g.groups < 256 && g.groups < need) g.groups *= 2;  // up to 4 KB of a 16-bit row in one piece
   g.col_ctas = (int)((need + g.groups - 1) / g.groups);
   const int strands = 256 / g.groups;
-  int64_t rows = (148 * 8 + g.col_ctas - 1) / g.col_ctas;  // about eight CTAs an SM
+  int64_t rows = (148 * 4) / g.col_ctas;  // four CTAs an SM at 64 registers a thread: one wave
   const int64_t most = (M + 2 * strands - 1) / (2 * strands);
   if (rows > most) rows = most;
   if (rows < 1) rows = 1;
   g.rows_per_cta = (M + rows - 1) / rows;
   g.row_ctas = (int)((M + g.rows_per_cta - 1) / g.rows_per_cta);
   return g;
+}
+
+// Rows of `cols` elements E copied to rows `ld` elements apart (a multiple of 16 bytes), zeros behind
+// them.  One 16-byte unit of the copy per thread: its elements are read one by one, which neighbouring
+// threads find in L1, and written at once.
+template <class E>
+__global__ void __launch_bounds__(256) pad_rows_kernel(const E* __restrict__ src, int64_t units, int cols, int units_per_row,
+                                                       uint4* __restrict__ dst) {
+  constexpr int V = 16 / (int)sizeof(E);
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= units) return;
+  const int64_t row = i / units_per_row;
+  const int c0 = (int)(i - row * units_per_row) * V;
+  const E* const at = src + row * cols + c0;
+  union { E e[V]; uint4 q; } o;
+#pragma unroll
+  for (int j = 0; j < V; ++j) o.e[j] = c0 + j < cols ? at[j] : E(0);
+  dst[i] = o.q;
 }
 
 int check_sizes(const char* what, int64_t M, int64_t N, int64_t K) {
@@ -307,11 +339,33 @@ extern "C" int gnn_linear_wgrad(const void* gz, int64_t ldg, const void* x, int6
   if (dtype == GNN_F32) {
     if (ldg != N || ldx != K) return fail(GNN_ERR_UNSUPPORTED, what, "fp32 rows must lie one after the other");
     return tf32x3_product_tn(static_cast<const float*>(gz), static_cast<const float*>(x), static_cast<float*>(grad_w), M, N,
-                             K, workspace, workspace_bytes, status, stream, kChain32);
+                             K, workspace, workspace_bytes, status, stream, kChain32Long);
   }
   const TcOperand a{gz, ldg, true}, b{x, ldx, true};
   if (!tma_operand_ok(a, 2) || !tma_operand_ok(b, 2))
     return fail(GNN_ERR_UNSUPPORTED, what, "rows must start on 16-byte boundaries");
   const LinearEpilogue ep{nullptr, nullptr, nullptr, nullptr, GNN_ACT_NONE, 0.f, nullptr, grad_w, dtype};
   return launch_linear_tc(a, b, dtype, N, K, M, ep, workspace, workspace_bytes, status, stream, what);
+}
+
+extern "C" int gnn_pad_rows(const void* src, int element_bytes, int64_t rows, int64_t cols, void* dst, int64_t ld,
+                            cudaStream_t stream) {
+  const char* const what = "gnn_pad_rows";
+  if (int rc = check_sizes(what, rows, cols, 1)) return rc;
+  if (element_bytes != 1 && element_bytes != 2 && element_bytes != 4)
+    return fail(GNN_ERR_UNSUPPORTED, what, "elements of 1, 2 or 4 bytes");
+  if (ld < cols || ld >= (1LL << 31) || ld * element_bytes % 16)
+    return fail(GNN_ERR_INVALID_ARG, what, "ld must hold the columns in whole 16-byte units");
+  if (rows == 0) return GNN_OK;
+  if (!src || !dst || (uintptr_t)dst % 16 || (uintptr_t)src % element_bytes)
+    return fail(GNN_ERR_INVALID_ARG, what, "null or misaligned pointer");
+  const int64_t per_row = ld * element_bytes / 16, units = rows * per_row, grid = (units + 255) / 256;
+  if (grid > INT32_MAX) return fail(GNN_ERR_LIMIT, what, "too many elements");
+  if (element_bytes == 4)
+    pad_rows_kernel<<<(unsigned)grid, 256, 0, stream>>>((const uint32_t*)src, units, (int)cols, (int)per_row, (uint4*)dst);
+  else if (element_bytes == 2)
+    pad_rows_kernel<<<(unsigned)grid, 256, 0, stream>>>((const uint16_t*)src, units, (int)cols, (int)per_row, (uint4*)dst);
+  else
+    pad_rows_kernel<<<(unsigned)grid, 256, 0, stream>>>((const uint8_t*)src, units, (int)cols, (int)per_row, (uint4*)dst);
+  return check_launch(what);
 }

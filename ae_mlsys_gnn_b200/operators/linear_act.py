@@ -37,17 +37,15 @@ def _status(dev):
 
 def _operand(t):
     """(tensor, row pitch in elements) of a contiguous matrix as the product kernels read it: rows a
-    multiple of 16 bytes apart that start on a 16-byte boundary; others are copied to such a pitch (for
-    fp32 the columns behind the last are zeros, which the reduction runs over)."""
-    k = t.shape[1]
-    per = 16 // t.element_size()
+    multiple of 16 bytes apart that start on a 16-byte boundary; others are copied to such a pitch, with
+    zeros behind the columns (in fp32 the reduction runs over them)."""
+    k, size = t.shape[1], t.element_size()
+    per = 16 // size
     if k % per == 0:
         return (t if t.data_ptr() % 16 == 0 else t.clone()), k
     ld = -(-k // per) * per
     buf = torch.empty((t.shape[0], ld), dtype=t.dtype, device=t.device)
-    buf[:, :k] = t
-    if t.dtype == torch.float32:
-        buf[:, k:] = 0
+    capi.launch(t.device, "gnn_pad_rows", t.data_ptr(), size, t.shape[0], k, buf.data_ptr(), ld)
     return buf, ld
 
 
@@ -78,7 +76,8 @@ class _LinearAct(torch.autograd.Function):
         # bias and activation share their pass of the backward; without an activation z is not needed
         need_z = act != 0 and any(ctx.needs_input_grad[:3])
         y, z = _forward((xo, ldx, x.shape[1]), None, (wo, ldw), None, bias, act, residual, slope, x.dtype, need_z)
-        ctx.save_for_backward(xo, wo, z)
+        # the fp32 products take any row pitch of the weights, the others read them by TMA
+        ctx.save_for_backward(xo, weight if x.dtype is torch.float32 else wo, z)
         ctx.args = (x.shape, act, slope)
         return y
 
@@ -108,18 +107,12 @@ class _LinearAct(torch.autograd.Function):
         if need_x:
             gx = torch.empty((M, K), dtype=dt, device=dev)
             if M:
-                wr, n, k, out = w, N, K, gx
-                if code == 0:  # the reduction runs over zero columns of gz, the output over those of w
-                    n, k = ldz, w.shape[1]
-                    if n != N:
-                        wr = torch.nn.functional.pad(w, (0, 0, 0, n - N))
-                    if k != K:
-                        out = torch.empty((M, k), dtype=dt, device=dev)
-                scratch, nbytes = capi.scratch("gnn_linear_dgrad_workspace_bytes", dev, M, n, k, code)
-                capi.launch(dev, "gnn_linear_dgrad", gz.data_ptr(), ldz, wr.data_ptr(), wr.shape[1], code, out.data_ptr(),
-                            M, n, k, capi.ptr(scratch), nbytes, _status(dev).data_ptr())
-                if out is not gx:
-                    gx.copy_(out[:, :K])
+                wr, n = w, N
+                if code == 0 and ldz != N:  # the reduction runs over the zero columns of gz
+                    wr, n = torch.nn.functional.pad(w, (0, 0, 0, ldz - N)), ldz
+                scratch, nbytes = capi.scratch("gnn_linear_dgrad_workspace_bytes", dev, M, n, K, code)
+                capi.launch(dev, "gnn_linear_dgrad", gz.data_ptr(), ldz, wr.data_ptr(), wr.shape[1], code, gx.data_ptr(),
+                            M, n, K, capi.ptr(scratch), nbytes, _status(dev).data_ptr())
         if need_w:
             gw = torch.empty((N, K), dtype=dt, device=dev)
             n, k, out = N, K, gw

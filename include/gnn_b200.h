@@ -518,7 +518,7 @@ int gnn_expert_combine_bwd(const void* grad_out, const void* rows, const void* w
  *   z = x_scale[m] * w_scale[n] * (x w^T) + bias,   y = act(z) + residual
  * x and w are fp32 (error-compensated 3xTF32, rows K elements apart, K % 4 == 0), bf16, fp16 or
  * e4m3 (in_type; rows ldx / ldw elements apart, each on a 16-byte boundary); the scales (one per
- * row of x and of w) belong to e4m3 operands alone.  bias, residual, y and z are of out_type (= in_type
+ * row of x and of w) belong to e4m3 operands alone.  Rows may be read up to the next 16-byte boundary.  bias, residual, y and z are of out_type (= in_type
  * except for e4m3); bias, residual and z may be NULL.  z is what the gradient needs of the forward
  * pass.  Sums and epilogue are fp32.  `status` as in gnn_gemm_tf32x3. */
 int gnn_linear_fwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int in_type, size_t* bytes);
@@ -534,6 +534,12 @@ int gnn_linear_act_bwd_workspace_bytes(int64_t M, int64_t N, int64_t ldz, size_t
 int gnn_linear_act_bwd(const void* grad_y, const void* z, int act, float slope, int dtype, int64_t M, int64_t N,
                        void* gz, int64_t ldz, void* grad_b, void* workspace, size_t workspace_bytes,
                        cudaStream_t stream);
+
+/* Copies rows of `cols` elements (of 1, 2 or 4 bytes) to rows ld elements apart, ld * element_bytes
+ * a multiple of 16 and dst on a 16-byte boundary; the elements behind the columns are zeroed.  This is
+ * how operands whose rows do not start on 16-byte boundaries are laid out for the products. */
+int gnn_pad_rows(const void* src, int element_bytes, int64_t rows, int64_t cols, void* dst, int64_t ld,
+                 cudaStream_t stream);
 
 /* Its products: grad_x [M,K] = gz w and grad_w [N,K] = gz^T x, fp32, bf16 or fp16; operand rows as
  * in gnn_linear_fwd (fp32: gz rows N elements apart, for grad_x N % 4 == 0). */

@@ -63,7 +63,7 @@ def test_sort_is_exact(cuda, t, k, e, d, dropped):
         assert torch.equal(order.offsets.cpu(), offsets) and torch.equal(order.slots.cpu(), slots)
 
 
-@pytest.mark.parametrize("pairs,e", [(2048, 3), (2049, 1), (4096, 1024), (65536, 8), (303105, 128), (1000003, 1000),
+@pytest.mark.parametrize("pairs,e", [(1024, 3), (1025, 2), (2048, 3), (2049, 1), (4096, 1024), (65536, 8), (303105, 128), (1000003, 1000),
                                      (2600000, 64)])
 def test_sort_of_many_pairs(cuda, pairs, e):
     """Several chunks, ids out of range on both sides, one expert far ahead of the others."""

@@ -46,7 +46,7 @@ def test_experts_c_refusals():
     lib = _capi.lib()
     need = ctypes.c_size_t(1)
     size = lambda n, e: lib.gnn_expert_sort_workspace_bytes(n, e, ctypes.byref(need))
-    assert size(2048, 64) == 0 and need.value == 0  # one chunk: no scratch
+    assert size(1024, 64) == 0 and need.value == 0  # one chunk: no scratch
     assert size(1 << 20, 64) == 0 and 0 < need.value <= 148 * 64 * 4 + 16
     assert size(-1, 64) == -1 and size(5, 0) == -1
     sort = lambda n=1 << 20, e=64, ids=ONE, ws=ONE, nb=1 << 30: lib.gnn_expert_sort(ids, 0, n, e, ONE, ONE, ws, nb, None)
@@ -108,6 +108,17 @@ def test_linear_c_refusals():
     for f in (dg, wg):
         assert f(gz=None) == -1 and f(ldg=7) == -1 and f(ldg=12) == -4 and f(dt=3) == -4
         assert f(dt=F32) == -3 and f(dt=F32, ldg=12) == -4
+
+
+def test_pad_rows_c_refusals():
+    from ae_mlsys_gnn_b200 import _capi
+
+    lib = _capi.lib()
+    pad = lambda src=ONE, size=2, rows=4, cols=5, dst=ONE, ld=8: lib.gnn_pad_rows(src, size, rows, cols, dst, ld, None)
+    assert pad(rows=0) == 0
+    assert pad(src=None) == -1 and pad(dst=None) == -1 and pad(dst=ctypes.c_void_p(264)) == -1
+    assert pad(src=ctypes.c_void_p(257)) == -1 and pad(ld=4) == -1 and pad(ld=12) == -1
+    assert pad(size=8) == -4 and pad(rows=-1) == -1 and pad(cols=0) == -1
 
 
 def test_linear_refuses_cpu_tensors():
