@@ -544,14 +544,30 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_
                               __uint_as_float(r[4 * j + 3]));
             __syncwarp();
             const float* const flat = reinterpret_cast<const float*>(stg);
-            const int top = t.m0 + lg * 32;
-            if (col0 + lane < p.N) {
-#pragma unroll 4
-              for (int rr = 0; rr < 32; ++rr)
-                if (top + rr < p.M) {
-                  const int64_t at = (int64_t)(top + rr) * p.ldc + col0 + lane;
-                  Cout[at] = finish_one(p.fin, at, col0 + lane, flat[(rr * 8 + ((lane >> 2) ^ (rr & 7))) * 4 + (lane & 3)]);
+            const int top = t.m0 + lg * 32, rows = min(32, p.M - top), col = col0 + lane;
+            const int unit = lane >> 2, word = lane & 3;
+            if (col < p.N) {
+              int64_t at = (int64_t)top * p.ldc + col;
+              if (!p.fin.bias && !p.fin.z && !p.fin.act && !p.fin.residual) {
+                if (rows == 32) {
+#pragma unroll
+                  for (int r0 = 0; r0 < 32; r0 += 8) {
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = flat[((r0 + i) * 8 + (unit ^ i)) * 4 + word];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) Cout[at + i * p.ldc] = v[i];
+                    at += 8 * p.ldc;
+                  }
+                } else {
+#pragma unroll 1
+                  for (int rr = 0; rr < rows; ++rr, at += p.ldc) Cout[at] = flat[(rr * 8 + (unit ^ (rr & 7))) * 4 + word];
                 }
+              } else {
+#pragma unroll 2
+                for (int rr = 0; rr < rows; ++rr, at += p.ldc)
+                  Cout[at] = finish_one(p.fin, at, col, flat[(rr * 8 + (unit ^ (rr & 7))) * 4 + word]);
+              }
             }
             __syncwarp();  // the block is rewritten by the next chunk
           } else if (last && row < p.M) {
