@@ -36,13 +36,13 @@ struct RowParts {
 };
 
 template <class T, int VEC, int NV, int MAXT>
-__global__ void __launch_bounds__(MAXT, sizeof(T) * VEC * NV <= 16 ? 2 : 1) rms_norm_bwd_kernel(const BwdParams p) {
+__global__ void __launch_bounds__(MAXT, MAXT == 512 && sizeof(T) * VEC * NV <= 16 ? 2 : 1) rms_norm_bwd_kernel(const BwdParams p) {
   __shared__ float s_sum[2][32];
   extern __shared__ float s_gw[];  // [d], groups within one warp only
   using P = Pack<T, VEC>;
   // Narrow shares are requested one row ahead and keep their weights in registers; for wide ones
   // (32 elements a thread) the registers do not suffice, and more bytes are in flight anyway.
-  constexpr bool kAhead = NV * VEC <= 16, kKeepWeight = NV * VEC <= 8;
+  constexpr bool kAhead = NV * VEC <= 8, kKeepWeight = kAhead;
   const int G = p.group;
   const int local = threadIdx.x / G, t = threadIdx.x - local * G;
   const int rows = blockDim.x / G;
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(1024) weight_grad_kernel(const float* __restri
 }
 
 NormGeom pick_bwd(int64_t d, int vec) {
-  NormGeom g = norm_geom(d, vec, norm_ept(d), 4);
+  NormGeom g = norm_geom(d, vec, norm_ept(d, false), 4);
   if (g.group <= 128) {  // several rows side by side
     g.rows = 256 / g.group;
     g.threads = g.rows * g.group;
@@ -235,11 +235,11 @@ extern "C" int gnn_rms_norm_bwd(const void* grad_y, const void* grad_h, const vo
   const int64_t want = (n + g.rows - 1) / g.rows;
   const int grid = (int)(want < kBwdCtas ? want : kBwdCtas);
   const size_t smem = g.rows > 1 ? (size_t)d * sizeof(float) : 0;
-  dispatch_norm(dtype, vec, g.ept, [&](auto tag, auto v, auto nv) {
+  dispatch_norm<false>(dtype, vec, g.ept, [&](auto tag, auto v, auto nv) {
     using T = decltype(tag);
     constexpr int V = decltype(v)::value, NV = decltype(nv)::value;
     if (g.threads <= 512) rms_norm_bwd_kernel<T, V, NV, 512><<<grid, g.threads, smem, stream>>>(p);
-    else if constexpr (V * NV == 32) rms_norm_bwd_kernel<T, V, NV, 1024><<<grid, g.threads, smem, stream>>>(p);
+    else rms_norm_bwd_kernel<T, V, NV, 1024><<<grid, g.threads, smem, stream>>>(p);
   });
   if (grad_w) {
     const dim3 block(32, 32);

@@ -32,7 +32,7 @@ struct FwdParams {
 };
 
 template <class T, int VEC, int NV, bool FP8, int MAXT>
-__global__ void __launch_bounds__(MAXT, sizeof(T) * VEC * NV <= 16 ? 4 : 1) rms_norm_kernel(const FwdParams p) {
+__global__ void __launch_bounds__(MAXT, MAXT == 512 && sizeof(T) * VEC * NV <= 16 ? 4 : 1) rms_norm_kernel(const FwdParams p) {
   __shared__ float s_sum[32];
   __shared__ int s_max[32];
   extern __shared__ int s_block_max[];  // [rows of this CTA][n_blocks], FP8 with block scales
@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(MAXT, sizeof(T) * VEC * NV <= 16 ? 4 : 1) rms_
 
 template <bool FP8>
 int launch_fwd(FwdParams p, int dtype, int vec, cudaStream_t stream, const char* what) {
-  const NormGeom g = norm_geom(p.d, vec, norm_ept(p.d), FP8 ? 32 : 4);
+  const NormGeom g = norm_geom(p.d, vec, norm_ept(p.d, vec * dtype_bytes(dtype) == 16), FP8 ? 32 : 4);
   p.group = g.group;
   const int64_t grid = (p.n + g.rows - 1) / g.rows;
   if (grid > INT32_MAX) {
@@ -170,11 +170,13 @@ int launch_fwd(FwdParams p, int dtype, int vec, cudaStream_t stream, const char*
     return GNN_ERR_LIMIT;
   }
   const size_t smem = FP8 && p.block ? (size_t)g.rows * p.n_blocks * sizeof(int) : 0;
-  dispatch_norm(dtype, vec, g.ept, [&](auto tag, auto v, auto nv) {
+  dispatch_norm<true>(dtype, vec, g.ept, [&](auto tag, auto v, auto nv) {
     using T = decltype(tag);
     constexpr int V = decltype(v)::value, NV = decltype(nv)::value;
-    if (g.threads <= 512) rms_norm_kernel<T, V, NV, FP8, 512><<<(unsigned)grid, g.threads, smem, stream>>>(p);
-    else if constexpr (V * NV == 32) rms_norm_kernel<T, V, NV, FP8, 1024><<<(unsigned)grid, g.threads, smem, stream>>>(p);
+    // with whole 16-byte accesses 8 or 16 elements a thread never need more than 512 threads
+    constexpr bool kNarrowOnly = V * sizeof(T) == 16 && V * NV < 32;
+    if (kNarrowOnly || g.threads <= 512) rms_norm_kernel<T, V, NV, FP8, 512><<<(unsigned)grid, g.threads, smem, stream>>>(p);
+    else if constexpr (!kNarrowOnly) rms_norm_kernel<T, V, NV, FP8, 1024><<<(unsigned)grid, g.threads, smem, stream>>>(p);
   });
   return check_launch(what);
 }
