@@ -248,15 +248,6 @@ __device__ __forceinline__ TileCoord decode_tile(const Params& p, int tile) {
   return t;
 }
 
-// The epilogue of one element at offset `at` of C.
-__device__ __forceinline__ float finish_one(const GemmFinish& f, int64_t at, int col, float v) {
-  if (f.bias) v += __ldg(f.bias + col);
-  if (f.z) f.z[at] = v;
-  v = act_value<true>(v, f.act, f.slope);
-  if (f.residual) v += __ldg(f.residual + at);
-  return v;
-}
-
 // FINISH: the epilogue of a linear layer (GemmFinish).  An instantiation of its own, so that the
 // plain product's epilogue keeps its registers.
 template <int BN, bool FINISH>
@@ -564,9 +555,26 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_
                   for (int rr = 0; rr < rows; ++rr, at += p.ldc) Cout[at] = flat[(rr * 8 + (unit ^ (rr & 7))) * 4 + word];
                 }
               } else {
-#pragma unroll 2
-                for (int rr = 0; rr < rows; ++rr, at += p.ldc)
-                  Cout[at] = finish_one(p.fin, at, col, flat[(rr * 8 + (unit ^ (rr & 7))) * 4 + word]);
+                const GemmFinish& f = p.fin;
+                const float bias = f.bias ? __ldg(f.bias + col) : 0.f;
+#pragma unroll 1
+                for (int r0 = 0; r0 < rows; r0 += 8, at += 8 * p.ldc) {
+                  float v[8], res[8];
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) {
+                    v[i] = flat[((r0 + i) * 8 + (unit ^ i)) * 4 + word] + bias;
+                    res[i] = f.residual && r0 + i < rows ? __ldg(f.residual + at + i * p.ldc) : 0.f;
+                  }
+                  if (f.z) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                      if (r0 + i < rows) f.z[at + i * p.ldc] = v[i];
+                  }
+                  apply_act<true>(v, f.act, f.slope);
+#pragma unroll
+                  for (int i = 0; i < 8; ++i)
+                    if (r0 + i < rows) Cout[at + i * p.ldc] = v[i] + res[i];
+                }
               }
             }
             __syncwarp();  // the block is rewritten by the next chunk

@@ -60,10 +60,11 @@ int launch_gemm_persistent(const GemmOperand& a, const GemmOperand& b, int64_t K
                            const GemmScores* scores = nullptr, const GemmFinish* finish = nullptr, int chain_kb = 0);
 
 // gnn_gemm_tf32x3 and gnn_gemm_tf32x3_tn (gemm_tf32x3.cu) with a linear layer's epilogue and a
-// chain length of choice; `what` names the entry point in error messages.
+// chain length of choice; `what` names the entry point in error messages.  splits > 1 (without scores):
+// the ranges' sums go to `planes` ([splits][M][N], the finish is not applied) instead of C.
 int tf32x3_product(const float* A, const float* B, int b_is_n_by_k, float* C, int64_t M, int64_t N, int64_t K,
                    void* workspace, size_t workspace_bytes, int* status, cudaStream_t stream, const GemmScores* scores,
-                   const GemmFinish* finish, int chain_kb, const char* what);
+                   const GemmFinish* finish, int chain_kb, const char* what, int splits = 1, float* planes = nullptr);
 int tf32x3_product_tn(const float* A, const float* B, float* C, int64_t M, int64_t K1, int64_t N1, void* workspace,
                       size_t workspace_bytes, int* status, cudaStream_t stream, int chain_kb);
 

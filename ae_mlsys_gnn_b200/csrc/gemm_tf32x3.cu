@@ -135,7 +135,7 @@ namespace gnn {
 
 int tf32x3_product(const float* A, const float* B, int b_is_n_by_k, float* C, int64_t M, int64_t N, int64_t K,
                    void* workspace, size_t workspace_bytes, int* status, cudaStream_t stream, const GemmScores* scores,
-                   const GemmFinish* finish, int chain_kb, const char* what) {
+                   const GemmFinish* finish, int chain_kb, const char* what, int splits, float* planes) {
   if (M < 0 || N < 0 || K < 0) return bad("gnn_gemm_tf32x3: negative size");
   if (M == 0 || N == 0) return GNN_OK;
   if (!A || !B || !C || !status) return bad("gnn_gemm_tf32x3: null pointer");
@@ -162,7 +162,9 @@ int tf32x3_product(const float* A, const float* B, int b_is_n_by_k, float* C, in
   }
   const GemmOperand oa{kKMajorRaw, A, nullptr, M};
   const GemmOperand ob{kKMajorSplit, b_hi, b_lo, N};
-  const int rc = launch_gemm_persistent(oa, ob, K, C, N, 1, 0, status, stream, scores, finish, chain_kb);
+  const GemmFinish plain{};
+  const int rc = splits > 1 ? launch_gemm_persistent(oa, ob, K, planes, N, splits, M * N, status, stream, nullptr, &plain, chain_kb)
+                            : launch_gemm_persistent(oa, ob, K, C, N, 1, 0, status, stream, scores, finish, chain_kb);
   if (rc != GNN_OK) return rc;
   return check_launch(what);
 }

@@ -185,6 +185,36 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const E* __restrict__ src
   dst[i] = o.q;
 }
 
+// fp32 products with few output tiles: ranges of the reduction axis, at least eight blocks of 32 each, so
+// that the SMs are occupied (106 x 6592 -> 47 is a single tile: 147 us without).
+int f32_splits(int64_t M, int64_t N, int64_t K) {
+  const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128), kb = (K + 31) / 32;
+  int64_t s = 148 / tiles;
+  if (s > kb / 8) s = kb / 8;
+  return s < 2 ? 1 : (int)s;
+}
+size_t f32_product_bytes(int64_t M, int64_t N, int64_t K) {  // of the weights' halves, then the planes
+  size_t bytes = 0;
+  gnn_gemm_tf32x3_workspace_bytes(M, N, K, &bytes);
+  bytes = (bytes + 255) / 256 * 256;
+  const int s = f32_splits(M, N, K);
+  return bytes + (s > 1 ? (size_t)s * M * N * sizeof(float) + 256 : 0);
+}
+int f32_product(const float* a, const float* b, int b_is_n_by_k, float* c, int64_t M, int64_t N, int64_t K,
+                const GemmFinish& fin, void* workspace, size_t workspace_bytes, int* status, cudaStream_t stream, const char* what) {
+  if (!workspace || workspace_bytes < f32_product_bytes(M, N, K)) return fail(GNN_ERR_WORKSPACE, what, "workspace too small");
+  const int splits = f32_splits(M, N, K);
+  size_t halves = 0;
+  gnn_gemm_tf32x3_workspace_bytes(M, N, K, &halves);
+  float* const planes = (float*)(((uintptr_t)workspace + (halves + 255) / 256 * 256 + 255) & ~(uintptr_t)255);
+  const int rc = tf32x3_product(a, b, b_is_n_by_k, c, M, N, K, workspace, halves, status, stream, nullptr, &fin, kChain32, what,
+                                splits, planes);
+  if (rc != GNN_OK || splits == 1) return rc;
+  const LinearEpilogue ep{nullptr, nullptr, fin.bias, fin.z, fin.act, fin.slope, fin.residual, c, GNN_F32};
+  launch_split_epilogue(planes, splits, M, N, ep, stream);
+  return check_launch(what);
+}
+
 int check_sizes(const char* what, int64_t M, int64_t N, int64_t K) {
   if (M < 0 || N < 1 || K < 1) return fail(GNN_ERR_INVALID_ARG, what, "bad size");
   if (M >= (1LL << 31) || N >= (1LL << 31) || K >= (1LL << 31)) return fail(GNN_ERR_LIMIT, what, "size exceeds int32");
@@ -203,8 +233,7 @@ extern "C" int gnn_linear_fwd_workspace_bytes(int64_t M, int64_t N, int64_t K, i
     return fail(GNN_ERR_INVALID_ARG, "gnn_linear_fwd_workspace_bytes", "bad argument");
   *bytes = 0;
   if (linear_few_wanted(M, N, K, in_type) || linear_narrow_wanted(M, K, in_type)) return GNN_OK;
-  if (in_type == GNN_F32) return gnn_gemm_tf32x3_workspace_bytes(M, N, K, bytes);
-  *bytes = linear_tc_workspace(M, N, K, in_type);
+  *bytes = in_type == GNN_F32 ? f32_product_bytes(M, N, K) : linear_tc_workspace(M, N, K, in_type);
   return GNN_OK;
 }
 
@@ -230,8 +259,9 @@ extern "C" int gnn_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t
     }
     const GemmFinish fin{static_cast<const float*>(bias), static_cast<float*>(z), act, slope,
                          static_cast<const float*>(residual)};
-    return tf32x3_product(static_cast<const float*>(x), static_cast<const float*>(w), 1, static_cast<float*>(y), M, N, K,
-                          workspace, workspace_bytes, status, stream, nullptr, &fin, kChain32, what);
+    if (K % 4 || (uintptr_t)x % 16) return fail(GNN_ERR_UNSUPPORTED, what, "fp32 rows must start on 16-byte boundaries");
+    return f32_product(static_cast<const float*>(x), static_cast<const float*>(w), 1, static_cast<float*>(y), M, N, K, fin,
+                       workspace, workspace_bytes, status, stream, what);
   }
   const TcOperand a{x, ldx, false}, b{w, ldw, false};
   const int elt = in_type == GNN_E4M3 ? 1 : 2;
@@ -289,8 +319,7 @@ extern "C" int gnn_linear_act_bwd(const void* grad_y, const void* z, int act, fl
 extern "C" int gnn_linear_dgrad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, size_t* bytes) {
   if (!bytes || M < 0 || N < 1 || K < 1 || !is_float(dtype))
     return fail(GNN_ERR_INVALID_ARG, "gnn_linear_dgrad_workspace_bytes", "bad argument");
-  if (dtype == GNN_F32) return gnn_gemm_tf32x3_workspace_bytes(M, K, N, bytes);
-  *bytes = linear_tc_workspace(M, K, N, dtype);
+  *bytes = dtype == GNN_F32 ? f32_product_bytes(M, K, N) : linear_tc_workspace(M, K, N, dtype);
   return GNN_OK;
 }
 
@@ -305,9 +334,9 @@ extern "C" int gnn_linear_dgrad(const void* gz, int64_t ldg, const void* w, int6
   if (ldg < N || ldw < K) return fail(GNN_ERR_INVALID_ARG, what, "a row is shorter than its columns");
   if (dtype == GNN_F32) {
     if (ldg != N || ldw != K) return fail(GNN_ERR_UNSUPPORTED, what, "fp32 rows must lie one after the other");
-    const GemmFinish plain{};
-    return tf32x3_product(static_cast<const float*>(gz), static_cast<const float*>(w), 0, static_cast<float*>(grad_x), M, K,
-                          N, workspace, workspace_bytes, status, stream, nullptr, &plain, kChain32, what);
+    if (N % 4 || (uintptr_t)gz % 16) return fail(GNN_ERR_UNSUPPORTED, what, "fp32 rows must start on 16-byte boundaries");
+    return f32_product(static_cast<const float*>(gz), static_cast<const float*>(w), 0, static_cast<float*>(grad_x), M, K, N,
+                       GemmFinish{}, workspace, workspace_bytes, status, stream, what);
   }
   const TcOperand a{gz, ldg, false}, b{w, ldw, true};
   if (!tma_operand_ok(a, 2) || !tma_operand_ok(b, 2))

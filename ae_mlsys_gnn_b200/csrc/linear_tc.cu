@@ -408,14 +408,27 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         const bool ok = p.planes ? run(float{}, std::true_type{}) : run(T{}, std::false_type{});
         if (!ok) { s_failed = 1; break; }
       } else {
-        // rows that are not whole 16-byte units: 32 x 32 blocks through shared memory, then one element
-        // per lane and step, neighbours of a row on neighbouring lanes
+        // rows that are not whole 16-byte units: 32 x 32 blocks through shared memory, then a column per
+        // lane, whose residual is requested before the sums are fetched
         if (!warp_wait(acc_full_bar(buf), (count >> 1) & 1, &s_failed)) { s_failed = 1; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const float my_rs = FP8 && !p.planes && row < p.M ? __ldg(p.ep.row_scale + row) : 1.f;
+        const int rows = min(32, p.M - top);
 #pragma unroll 1
         for (int c = part; c < BN / 32; c += 2) {
-          const int col0 = t.n0 + c * 32;
-          if (col0 >= p.N || top >= p.M) break;
+          const int col0 = t.n0 + c * 32, col = col0 + lane;
+          if (col0 >= p.N || rows <= 0) break;
+          const bool in = col < p.N;
+          const int64_t at = (int64_t)top * p.N + col;
+          const bool with_r = p.ep.residual && !p.planes;
+          T res[32];
+          if (with_r) {
+            const T* const src = static_cast<const T*>(p.ep.residual) + (in ? at : 0);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) res[i] = src[(int64_t)(in ? min(i, rows - 1) : 0) * p.N];
+          }
+          const float bias = in && p.ep.bias && !p.planes ? to_f32(static_cast<const T*>(p.ep.bias)[col]) : 0.f;
+          const float cs = FP8 && in && !p.planes ? __ldg(p.ep.col_scale + col) : 1.f;
 #pragma unroll 1
           for (int q = 0; q < 2; ++q) {
             uint32_t r[16];
@@ -427,12 +440,31 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             RowPiece<float>::put(block, lane, q, v);
           }
           __syncwarp();
-          if (col0 + lane < p.N) {
-#pragma unroll 1
-            for (int rr = 0; rr < 32 && top + rr < p.M; ++rr) {
-              const float v = *reinterpret_cast<const float*>(block + rr * 128 + (((lane >> 2) ^ (rr & 7)) << 4) + (lane & 3) * 4);
-              if (p.planes) p.planes[((size_t)t.z * p.M + top + rr) * p.N + col0 + lane] = v;
-              else finish_one<T>(p.ep, top + rr, col0 + lane, p.N, v);
+#pragma unroll
+          for (int r0 = 0; r0 < 32; r0 += 8) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              v[i] = *reinterpret_cast<const float*>(block + (r0 + i) * 128 + (((lane >> 2) ^ i) << 4) + (lane & 3) * 4);
+              if constexpr (FP8) v[i] *= __shfl_sync(kFull, my_rs, r0 + i) * cs;
+              v[i] += bias;
+            }
+            if (p.planes) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (in && r0 + i < rows) p.planes[(size_t)t.z * p.M * p.N + at + (int64_t)(r0 + i) * p.N] = v[i];
+              continue;
+            }
+            if (p.ep.z) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (in && r0 + i < rows) static_cast<T*>(p.ep.z)[at + (int64_t)(r0 + i) * p.N] = from_f32<T>(v[i]);
+            }
+            apply_act<sizeof(T) == 4>(v, p.ep.act, p.ep.slope);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if (with_r) v[i] += to_f32(res[r0 + i]);
+              if (in && r0 + i < rows) static_cast<T*>(p.ep.out)[at + (int64_t)(r0 + i) * p.N] = from_f32<T>(v[i]);
             }
           }
           __syncwarp();  // the block is rewritten by the next chunk
