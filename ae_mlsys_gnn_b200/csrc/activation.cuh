@@ -36,9 +36,12 @@ __device__ __forceinline__ float act_one(float z, float slope) {
   else return z;
 }
 
-// act'(z); at the corner of relu and leaky_relu the slope of the negative side
+// act'(z); at the corner of relu and leaky_relu the slope of the negative side.  gelu and silu have
+// reached their limits long before |z| = 100; beyond it (a z that overflowed its 16-bit type, say)
+// products like infinity * 0 are kept out.
 template <int ACT, bool FINE>
 __device__ __forceinline__ float slope_one(float z, float slope) {
+  if constexpr (ACT == GNN_ACT_GELU || ACT == GNN_ACT_SILU) z = z > 100.f ? 100.f : z < -100.f ? -100.f : z;
   if constexpr (ACT == GNN_ACT_RELU) return z > 0.f ? 1.f : 0.f;
   else if constexpr (ACT == GNN_ACT_LEAKY_RELU) return z > 0.f ? 1.f : slope;
   else if constexpr (ACT == GNN_ACT_ELU) return z > 0.f ? 1.f : __expf(z);
@@ -49,7 +52,7 @@ __device__ __forceinline__ float slope_one(float z, float slope) {
     const float tail = normal_tail(z, gauss);
     return (z > 0.f ? 1.f - tail : tail) + z * 0.39894228040143268f * gauss;
   } else if constexpr (ACT == GNN_ACT_SILU) {
-    const float s = __fdividef(1.f, 1.f + __expf(-z));
+    const float s = __fdividef(1.f, 1.f + __expf(-z));  // __expf(100) overflows to infinity, s = 0
     return s * (1.f + z * (1.f - s));
   } else return 1.f;
 }

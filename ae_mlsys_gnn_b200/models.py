@@ -13,17 +13,24 @@ import torch
 from torch import nn
 
 from .layers import EdgeConv, GATConv, GMMConv
+from .operators.rms_norm import add_rms_norm
 
 
 class GAT(nn.Module):
     """Stack of GATConv layers; heads are concatenated between layers and averaged
     at the output.  ``activation`` (None or "elu") is applied between layers: the
     reference model stores an activation but never applies it
-    (train_gatconv_our.py:47-53); the benchmark configurations apply ELU."""
+    (train_gatconv_our.py:47-53); the benchmark configurations apply ELU.
+
+    ``norm="rms"`` (default None, as in the reference): the hidden layers' outputs run along a residual
+    stream, added to it where the width stays the same, and every next layer reads the stream's
+    root-mean-square norm (``operators.rms_norm.add_rms_norm``)."""
 
     def __init__(self, in_dim, hidden, heads, num_classes, out_heads=1, negative_slope=0.2,
-                 activation="elu"):
+                 activation="elu", norm=None):
         super().__init__()
+        if norm not in (None, "rms"):
+            raise ValueError("norm must be None or 'rms'")
         if isinstance(hidden, int):
             hidden = [hidden] * len(heads)
         dims_in = [in_dim] + [h * f for h, f in zip(heads, hidden)]
@@ -34,11 +41,15 @@ class GAT(nn.Module):
              for i in range(len(heads))])
         self.gat_layers.append(GATConv(dims_in[-1], num_classes, out_heads, negative_slope))
         self.activation = activation
+        self.norm_weights = nn.ParameterList([torch.ones(d) for d in dims_in[1:]]) if norm == "rms" else None
 
     def forward(self, row_ptr, col_ind, col_ptr, row_ind, inputs, save_memory=True):
-        h = inputs
-        for layer in self.gat_layers[:-1]:
+        h, stream = inputs, None
+        for i, layer in enumerate(self.gat_layers[:-1]):
             h = layer(row_ptr, col_ind, col_ptr, row_ind, h, save_memory).flatten(1)
+            if self.norm_weights is not None:
+                same = stream is not None and stream.shape == h.shape
+                h, stream = add_rms_norm(h, self.norm_weights[i], stream if same else None)
         out = self.gat_layers[-1](row_ptr, col_ind, col_ptr, row_ind, h, save_memory)
         # the mean over one output head is the head itself: a view, not a pass over N x F
         return out.squeeze(1) if out.shape[1] == 1 else out.mean(1)

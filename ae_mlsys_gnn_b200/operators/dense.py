@@ -93,7 +93,7 @@ def check_status(dev=None) -> None:
             continue
         if int(t.item()) != 0:
             t.zero_()
-            raise capi.GnnError("gnn_gemm_tf32x3: a barrier wait expired inside the kernel")
+            raise capi.GnnError("gnn_gemm_tf32x3 / gnn_linear: a barrier wait expired inside a product kernel")
 
 
 def supported(m: int, n: int, k: int, a: torch.Tensor) -> bool:

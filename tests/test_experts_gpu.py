@@ -251,3 +251,34 @@ def test_refusals(cuda):
         expert_combine(rows, w[:, :1], order)
     with pytest.raises(TypeError):
         expert_combine(rows, w.half(), order)
+
+
+def test_beyond_32_bit_offsets(cuda):
+    """More than 2^31 elements in expert order: rows at the far end go there and back."""
+    from ae_mlsys_gnn_b200.operators.experts import expert_combine, expert_dispatch, expert_sort
+
+    t, k, d, e = 66000, 8, 4160, 16
+    gen = torch.Generator(device=cuda).manual_seed(3)
+    ids = torch.rand(t, e, generator=gen, device=cuda).topk(k, 1).indices
+    order = expert_sort(ids, e)
+    x = torch.randn(t, d, generator=gen, device=cuda).to(torch.bfloat16).requires_grad_(True)
+    xs = expert_dispatch(x, order)
+    some = torch.arange(0, t, 997, device=cuda)
+    at = order.slots[some].long()
+    assert int(at.max()) * d > 2 ** 31
+    assert torch.equal(xs[at[:, 5]], x[some]) and torch.equal(xs[at[:, 0]], x[some])
+    w = torch.rand(t, k, generator=gen, device=cuda).requires_grad_(True)
+    out = expert_combine(xs, w, order)
+    want = x[some].double() * w[some].double().sum(1, keepdim=True)
+    within(out[some], want, half_step(torch.bfloat16) * 1.01 * want.abs() + 10 * U * x[some].double().abs() * k, "out")
+    g = torch.randn(t, d, generator=gen, device=cuda).to(torch.bfloat16)
+    gxs, gw = torch.autograd.grad(out, (xs, w), g, retain_graph=True)
+    assert torch.equal(gxs[at[:, 3]], (g[some].float() * w[some, 3:4]).to(torch.bfloat16))
+    want = (g[some].double() * x[some].double()).sum(1)
+    size = (g[some].double() * x[some].double()).abs().sum(1)
+    within(gw[some, 2], want, (d / 32 + 22) * U * size * 1.01, "grad_w")
+    gx, = torch.autograd.grad(xs, x, gxs)
+    want = g[some].double() * 0
+    for j in range(k):
+        want = want + gxs[at[:, j]].double()
+    within(gx[some], want, half_step(torch.bfloat16) * 1.01 * want.abs() + 10 * U * k * gxs[at].double().abs().amax(1), "grad_x")

@@ -278,6 +278,44 @@ def test_empty_and_special_values(cuda):
             assert bool(torch.isfinite(y).all()) and bool(torch.isfinite(torch.autograd.grad(y.sum(), lf)[0]).all())
 
 
+def test_slopes_where_z_overflowed(cuda):
+    """fp16 pre-activations of +-infinity: the activations' slopes are at their limits, 1 and 0."""
+    from ae_mlsys_gnn_b200.operators.linear_act import linear_act
+
+    w = torch.full((8, 64), 60000.0, dtype=torch.float16, device=cuda)
+    g = torch.ones(200, 8, dtype=torch.float16, device=cuda)
+    b = torch.zeros(8, dtype=torch.float16, device=cuda, requires_grad=True)
+    for sign, slope in ((1.0, 1.0), (-1.0, 0.0)):
+        x = torch.full((200, 64), sign, dtype=torch.float16, device=cuda)
+        for act in ("gelu", "silu", "relu", "elu"):
+            gb, = torch.autograd.grad(linear_act(x, w, b, act), b, g)
+            assert torch.equal(gb, torch.full_like(gb, 200 * slope))
+
+
+def test_beyond_32_bit_offsets(cuda):
+    """More than 2^31 elements in the output, its gradient and the saved pre-activation: the last rows
+    are those of a small call."""
+    from ae_mlsys_gnn_b200.operators import dense
+    from ae_mlsys_gnn_b200.operators.linear_act import linear_act
+
+    m, k, n = 270000, 64, 8192
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    x = torch.randn(m, k, generator=gen, device=cuda).to(torch.bfloat16).requires_grad_(True)
+    w = (torch.randn(n, k, generator=gen, device=cuda) / 8).to(torch.bfloat16).requires_grad_(True)
+    y = linear_act(x, w, None, "silu")
+    g = torch.zeros_like(y)
+    g[-300:] = torch.randn(300, n, generator=gen, device=cuda).to(torch.bfloat16)
+    gx, gw = torch.autograd.grad(y, (x, w), g)
+    dense.check_status()
+    xs = x[-300:].detach().clone().requires_grad_(True)
+    ys = linear_act(xs, w, None, "silu")
+    gxs, gws = torch.autograd.grad(ys, (xs, w), g[-300:].contiguous())
+    assert torch.equal(y[-300:], ys)
+    for a, b in ((gx[-300:], gxs), (gw, gws)):  # other splits of the sums, one rounding each
+        assert float((a.double() - b.double()).norm() / b.double().norm()) < 2 * half_step(torch.bfloat16)
+    assert not bool(gx[:-300].any())
+
+
 def test_parts_of_the_gradient(cuda):
     """Each leaf alone gives what all of them together give."""
     from ae_mlsys_gnn_b200.operators.linear_act import linear_act

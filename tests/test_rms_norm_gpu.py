@@ -257,3 +257,29 @@ def test_streams_and_graph(cuda):
     assert torch.equal(gy, y) and torch.equal(gh, h)
     q0, s0, _ = add_rms_norm_fp8(x, w, r)
     assert torch.equal(q.view(torch.uint8), q0.view(torch.uint8)) and torch.equal(s, s0)
+
+
+def test_beyond_32_bit_offsets(cuda):
+    """More than 2^31 elements: the last rows are those of a small call."""
+    from ae_mlsys_gnn_b200.operators.rms_norm import add_rms_norm, add_rms_norm_fp8
+
+    n, d = 530000, 4096
+    gen = torch.Generator(device=cuda).manual_seed(2)
+    x = torch.zeros(n, d, dtype=torch.bfloat16, device=cuda)
+    x[-9:] = torch.randn(9, d, generator=gen, device=cuda).to(torch.bfloat16)
+    w = torch.randn(d, generator=gen, device=cuda).to(torch.bfloat16)
+    lx, lw = x.requires_grad_(True), w.requires_grad_(True)
+    y, _ = add_rms_norm(lx, lw)
+    sx = x[-9:].detach().clone().requires_grad_(True)
+    ys, _ = add_rms_norm(sx, lw)
+    assert torch.equal(y[-9:], ys)
+    gy = torch.zeros_like(y)
+    gy[-9:] = torch.randn(9, d, generator=gen, device=cuda).to(torch.bfloat16)
+    gx, gw = torch.autograd.grad(y, (lx, lw), gy)
+    gxs, gws = torch.autograd.grad(ys, (sx, lw), gy[-9:].contiguous())
+    assert torch.equal(gx[-9:], gxs)
+    assert float((gw.double() - gws.double()).norm() / gws.double().norm()) < 2 * half_step(torch.bfloat16)
+    with torch.no_grad():
+        q, s, _ = add_rms_norm_fp8(x, w)
+        qs, ss, _ = add_rms_norm_fp8(sx, w)
+    assert torch.equal(q[-9:].view(torch.uint8), qs.view(torch.uint8)) and torch.equal(s[-9:], ss)
