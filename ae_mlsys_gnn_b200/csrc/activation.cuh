@@ -37,23 +37,23 @@ __device__ __forceinline__ float act_one(float z, float slope) {
 }
 
 // act'(z); at the corner of relu and leaky_relu the slope of the negative side.  gelu and silu have
-// reached their limits long before |z| = 100; beyond it (a z that overflowed its 16-bit type, say)
-// products like infinity * 0 are kept out.
+// reached their limits long before |z| = 100; beyond it (a z that overflowed its 16-bit type, say) the
+// products of z with a zero are kept finite.
 template <int ACT, bool FINE>
 __device__ __forceinline__ float slope_one(float z, float slope) {
-  if constexpr (ACT == GNN_ACT_GELU || ACT == GNN_ACT_SILU) z = z > 100.f ? 100.f : z < -100.f ? -100.f : z;
+  const float near = fminf(fmaxf(z, -100.f), 100.f);
   if constexpr (ACT == GNN_ACT_RELU) return z > 0.f ? 1.f : 0.f;
   else if constexpr (ACT == GNN_ACT_LEAKY_RELU) return z > 0.f ? 1.f : slope;
   else if constexpr (ACT == GNN_ACT_ELU) return z > 0.f ? 1.f : __expf(z);
   else if constexpr (ACT == GNN_ACT_GELU && FINE)
-    return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+    return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + near * 0.39894228040143268f * __expf(-0.5f * z * z);
   else if constexpr (ACT == GNN_ACT_GELU) {
     float gauss;
     const float tail = normal_tail(z, gauss);
-    return (z > 0.f ? 1.f - tail : tail) + z * 0.39894228040143268f * gauss;
+    return fmaf(near * 0.39894228040143268f, gauss, z > 0.f ? 1.f - tail : tail);
   } else if constexpr (ACT == GNN_ACT_SILU) {
-    const float s = __fdividef(1.f, 1.f + __expf(-z));  // __expf(100) overflows to infinity, s = 0
-    return s * (1.f + z * (1.f - s));
+    const float s = __fdividef(1.f, 1.f + __expf(-z));  // 0 where __expf overflows to infinity
+    return s * (1.f + near * (1.f - s));
   } else return 1.f;
 }
 

@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 #include "../../include/gnn_b200.h"
 
 namespace gnn {
@@ -26,9 +27,19 @@ struct alignas(VEC * sizeof(T)) Pack {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) o[i] = to_f32(v[i]);
   }
-  __device__ __forceinline__ void round(const float (&o)[VEC]) {
+  // Pairs are rounded by one instruction each.
+  __device__ __forceinline__ void round(const float (&o)[VEC]) { round_from(o); }
+  __device__ __forceinline__ void round_from(const float* o) {
+    if constexpr (VEC % 2 == 0 && std::is_same_v<T, __nv_bfloat16>) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = from_f32<T>(o[i]);
+      for (int i = 0; i < VEC; i += 2) reinterpret_cast<__nv_bfloat162*>(v)[i / 2] = __floats2bfloat162_rn(o[i], o[i + 1]);
+    } else if constexpr (VEC % 2 == 0 && std::is_same_v<T, __half>) {
+#pragma unroll
+      for (int i = 0; i < VEC; i += 2) reinterpret_cast<__half2*>(v)[i / 2] = __floats2half2_rn(o[i], o[i + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = from_f32<T>(o[i]);
+    }
   }
 };
 

@@ -91,8 +91,7 @@ __global__ void __launch_bounds__(256, 4) act_bwd_kernel(const ActBwdParams p) {
 #pragma unroll
             for (int i = 0; i < Q; ++i) {
               Pack<T, V> o;
-#pragma unroll
-              for (int j = 0; j < V; ++j) o.v[j] = from_f32<T>(v[i * V + j]);
+              o.round_from(v + i * V);
               store_pack(reinterpret_cast<Pack<T, V>*>(gz + row * p.ldz + col) + i, o);
             }
           }

@@ -23,8 +23,7 @@ __device__ __forceinline__ void store8(T* p, const float (&o)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; i += V) {
     Pack<T, V> a;
-#pragma unroll
-    for (int j = 0; j < V; ++j) a.v[j] = from_f32<T>(o[i + j]);
+    a.round_from(o + i);
     store_pack(reinterpret_cast<Pack<T, V>*>(p + i), a);
   }
 }

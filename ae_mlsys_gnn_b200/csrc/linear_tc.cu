@@ -165,8 +165,7 @@ struct RowPiece {
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
       Pack<O, V> o;
-#pragma unroll
-      for (int j = 0; j < V; ++j) o.v[j] = from_f32<O>(v[u * V + j]);
+      o.round_from(v + u * V);
       store_pack(reinterpret_cast<Pack<O, V>*>(at(block, lane, piece, u)), o);
     }
   }

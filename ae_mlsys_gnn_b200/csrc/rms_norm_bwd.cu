@@ -7,6 +7,7 @@
 // many rows, with the next row's loads in flight while the current one is reduced, and its threads
 // keep the weight gradient of their own columns in fp32 registers; the CTAs' sums go to a
 // workspace and a second kernel adds them in a fixed order, so the result is reproducible.
+#include <algorithm>
 #include <type_traits>
 #include "rms_norm.cuh"
 
@@ -35,8 +36,14 @@ struct RowParts {
   float rstd;
 };
 
+// CTAs of MAXT threads that an SM holds: what the registers of a kernel without spills allow (8
+// elements a thread: 85 for 16-bit rows, 112 for fp32).  16381 x 2048 bf16: 72.7 us at three CTAs of 256,
+// 87 us at two, 84 us at four whose 64 registers spill.
+template <class T, int EPT, int MAXT>
+constexpr int kResident = MAXT == 256 ? (sizeof(T) == 2 ? 3 : 2) : MAXT == 512 && sizeof(T) * EPT <= 16 ? 2 : 1;
+
 template <class T, int VEC, int NV, int MAXT>
-__global__ void __launch_bounds__(MAXT, MAXT == 512 && sizeof(T) * VEC * NV <= 16 ? 2 : 1) rms_norm_bwd_kernel(const BwdParams p) {
+__global__ void __launch_bounds__(MAXT, kResident<T, VEC * NV, MAXT>) rms_norm_bwd_kernel(const BwdParams p) {
   __shared__ float s_sum[2][32];
   extern __shared__ float s_gw[];  // [d], groups within one warp only
   using P = Pack<T, VEC>;
@@ -232,14 +239,20 @@ extern "C" int gnn_rms_norm_bwd(const void* grad_y, const void* grad_h, const vo
   const NormGeom g = pick_bwd(d, vec);
   float* const partial = grad_w ? (float*)(((uintptr_t)workspace + 15) & ~(uintptr_t)15) : nullptr;
   BwdParams p{grad_y, grad_h, h, weight, rstd, weight_dtype == GNN_F32 && dtype != GNN_F32, n, (int)d, g.group, grad_x, partial};
-  const int64_t want = (n + g.rows - 1) / g.rows;
-  const int grid = (int)(want < kBwdCtas ? want : kBwdCtas);
   const size_t smem = g.rows > 1 ? (size_t)d * sizeof(float) : 0;
+  int grid = 0;
   dispatch_norm<false>(dtype, vec, g.ept, [&](auto tag, auto v, auto nv) {
     using T = decltype(tag);
     constexpr int V = decltype(v)::value, NV = decltype(nv)::value;
-    if (g.threads <= 512) rms_norm_bwd_kernel<T, V, NV, 512><<<grid, g.threads, smem, stream>>>(p);
-    else rms_norm_bwd_kernel<T, V, NV, 1024><<<grid, g.threads, smem, stream>>>(p);
+    auto go = [&](auto kernel, int threads) {  // threads: resident on an SM
+      const int64_t want = (n + g.rows - 1) / g.rows, most = 148 * std::max(1, std::min(4, threads / g.threads));
+      grid = (int)std::min(want, most);
+      kernel<<<grid, g.threads, smem, stream>>>(p);
+    };
+    if constexpr (V * NV == 8)  // 32 elements a thread begin beyond 256 threads
+      if (g.threads <= 256) return go(rms_norm_bwd_kernel<T, V, NV, 256>, 256 * kResident<T, V * NV, 256>);
+    if (g.threads <= 512) go(rms_norm_bwd_kernel<T, V, NV, 512>, 512 * kResident<T, V * NV, 512>);
+    else go(rms_norm_bwd_kernel<T, V, NV, 1024>, 1024);
   });
   if (grad_w) {
     const dim3 block(32, 32);
