@@ -1,9 +1,9 @@
-// The linear layer for up to 128 rows of 16-bit or 8-bit elements: out = epilogue(x W^T), bound by the
+// The linear layer for up to 64 rows of 16-bit or 8-bit elements: out = epilogue(x W^T), bound by the
 // bytes of W.
 //
 // W is the 128-row operand of the tcgen05 MMA and the few rows of x are its N side, so a stage of the
-// TMA pipeline is 128 rows of W and only as many rows of x as there are (padded to 16, 32, 64 or
-// 128): up to 160 KB of W are in flight on every SM.  One CTA computes 128 columns of the output for
+// TMA pipeline is 128 rows of W and only as many rows of x as there are (padded to 16, 32 or
+// 64), and two CTAs of an SM keep up to 192 KB of W in flight.  One CTA computes 128 columns of the output for
 // all rows; where N / 128 leaves SMs idle, a cluster of CTAs divides the reduction axis and its partial
 // sums meet in distributed shared memory, added in a fixed order.  In the accumulator a lane of
 // tensor memory is a column of the output: consecutive lanes store consecutive columns, bias and the
@@ -21,6 +21,7 @@ constexpr int BM = 128;  // rows of W per CTA
 constexpr int kATile = BM * kStageK;
 constexpr int kThreads = 32 * 6;  // TMA, MMA, four epilogue warps
 constexpr int kMaxStages = 10;
+constexpr int kHalfSm = 114 * 1024;  // shared memory of a CTA when two share an SM
 constexpr int kNumBars = 2 * kMaxStages + 1;
 constexpr int kBarBytes = (8 * kNumBars + 16 + 127) / 128 * 128;
 constexpr int kMaxCluster = 8;
@@ -45,7 +46,7 @@ __device__ __forceinline__ float load_remote(uint32_t addr, uint32_t rank) {
 }
 
 template <int BN, bool FP8, class T>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, 2)
 linear_narrow_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const NarrowParams p) {
   constexpr int kStageBytes = kATile + BN * kStageK;
   constexpr int kTmemCols = BN < 32 ? 32 : BN;
@@ -209,11 +210,11 @@ int launch_instance(const CUtensorMap& mw, const CUtensorMap& mx, NarrowParams p
   constexpr int kStageBytes = kATile + BN * kStageK;
   auto kernel = linear_narrow_kernel<BN, FP8, T>;
   const int fixed = 1024 + kBarBytes;
-  p.stages = (kSmemLimit - 64 - fixed) / kStageBytes;
+  p.stages = (kHalfSm - fixed) / kStageBytes;
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   const int smem = fixed + p.stages * kStageBytes;
   static SmemGrant grant;
-  grant.allow(kernel, kSmemLimit - 64);
+  grant.allow(kernel, kHalfSm);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((p.N + BM - 1) / BM * p.cluster));
   cfg.blockDim = dim3(kThreads);
@@ -233,8 +234,7 @@ int launch_shape(int bn, const CUtensorMap& mw, const CUtensorMap& mx, const Nar
   switch (bn) {
     case 16: return launch_instance<16, FP8, T>(mw, mx, p, stream);
     case 32: return launch_instance<32, FP8, T>(mw, mx, p, stream);
-    case 64: return launch_instance<64, FP8, T>(mw, mx, p, stream);
-    default: return launch_instance<128, FP8, T>(mw, mx, p, stream);
+    default: return launch_instance<64, FP8, T>(mw, mx, p, stream);
   }
 }
 
@@ -242,7 +242,7 @@ int launch_shape(int bn, const CUtensorMap& mw, const CUtensorMap& mx, const Nar
 
 int launch_linear_narrow(const TcOperand& a, const TcOperand& b, int in_type, int64_t M, int64_t N, int64_t K,
                          const LinearEpilogue& ep, int* status, cudaStream_t stream, const char* what) {
-  const int bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  const int bn = M <= 16 ? 16 : M <= 32 ? 32 : 64;
   const bool fp8 = in_type == GNN_E4M3;
   CUtensorMap mw, mx;
   if (!encode_operand(&mw, b, in_type, N, K, BM) || !encode_operand(&mx, a, in_type, M, K, bn)) {
@@ -256,11 +256,11 @@ int launch_linear_narrow(const TcOperand& a, const TcOperand& b, int in_type, in
   p.N = (int)N;
   p.k_elems = fp8 ? kStageK : kStageK / 2;
   p.total_kb = (int)((K + p.k_elems - 1) / p.k_elems);
-  // CTAs of a cluster divide the reduction axis until the SMs are occupied, 4 stages each at least
+  // CTAs of a cluster divide the reduction axis until the SMs hold two each, 4 stages at least
   const int64_t tiles = (N + BM - 1) / BM;
   p.cluster = 1;
   while (p.cluster < kMaxCluster &&
-         ((tiles * p.cluster * 2 <= 148 && p.total_kb >= 8 * p.cluster) || p.total_kb > max_chain(in_type) * p.cluster))
+         ((tiles * p.cluster * 2 <= 2 * 148 && p.total_kb >= 8 * p.cluster) || p.total_kb > max_chain(in_type) * p.cluster))
     p.cluster *= 2;
   p.kb_per_cta = (p.total_kb + p.cluster - 1) / p.cluster;
   const uint32_t type = in_type == GNN_BF16 ? 1u : 0u;  // see launch_linear_tc
@@ -279,10 +279,12 @@ int launch_linear_narrow(const TcOperand& a, const TcOperand& b, int in_type, in
   return check_launch(what);
 }
 
-// Reductions of more than 8 of the longest chains go to linear_tc.cu, which splits them further.
+// From 65 rows on the row-by-row epilogue costs what the wide tile of linear_tc.cu costs (128 x 4096 x
+// 4096 bf16: 22 us both) and more for short reductions (128 x 1024 x 8192 e4m3: 31 against 19 us).
+// Reductions of more than 8 of the longest chains go there too, to be split further.
 bool linear_narrow_wanted(int64_t M, int64_t K, int in_type) {
   const int elt = in_type == GNN_E4M3 ? 1 : 2;
-  return in_type != GNN_F32 && M <= 128 && K * elt <= kMaxCluster * max_chain(in_type) * kStageK;
+  return in_type != GNN_F32 && M <= 64 && K * elt <= kMaxCluster * max_chain(in_type) * kStageK;
 }
 
 }  // namespace gnn

@@ -43,7 +43,7 @@ bool linear_few_wanted(int64_t M, int64_t N, int64_t K, int in_type);
 int launch_linear_few(const TcOperand& a, const TcOperand& b, int in_type, int64_t M, int64_t N, int64_t K,
                       const LinearEpilogue& ep, cudaStream_t stream, const char* what);
 
-// The same product for up to 128 rows of 16-bit or 8-bit operands (linear_narrow.cu), both K-major;
+// The same product for up to 64 rows of 16-bit or 8-bit operands (linear_narrow.cu), both K-major;
 // no workspace.
 bool linear_narrow_wanted(int64_t M, int64_t K, int in_type);
 int launch_linear_narrow(const TcOperand& a, const TcOperand& b, int in_type, int64_t M, int64_t N, int64_t K,

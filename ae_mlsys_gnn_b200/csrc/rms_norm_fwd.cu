@@ -152,8 +152,14 @@ __global__ void __launch_bounds__(MAXT, MAXT == 512 && sizeof(T) * VEC * NV <= 1
       if (col < p.d) {
         const float inv = 1.f / (p.block ? scale_of(bm[col / 128]) : row_scale);
         Pack<uint8_t, VEC> o;
+        if constexpr (VEC % 2 == 0) {  // pairs are rounded by one instruction each
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) o.v[j] = __nv_cvt_float_to_fp8(v[i][j] * inv, __NV_SATFINITE, __NV_E4M3);
+          for (int j = 0; j < VEC; j += 2)
+            reinterpret_cast<__nv_fp8x2_storage_t*>(o.v)[j / 2] =
+                __nv_cvt_float2_to_fp8x2(make_float2(v[i][j] * inv, v[i][j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+        } else {
+          o.v[0] = __nv_cvt_float_to_fp8(v[i][0] * inv, __NV_SATFINITE, __NV_E4M3);
+        }
         store_pack(reinterpret_cast<Pack<uint8_t, VEC>*>(p.q + row * p.d + col), o);
       }
     }
