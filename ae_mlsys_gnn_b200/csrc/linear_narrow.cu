@@ -9,6 +9,10 @@
 // tensor memory is a column of the output: consecutive lanes store consecutive columns, bias and the
 // weights' scale are one value per thread.
 //
+// Measured on a B200 (event time, of which about 6 us are the events): 19 x 4096 -> 8192 e4m3 (33.6
+// MB) 16.4 us, 64 rows 20.5 us; 64 x 4096 -> 32768 bf16 (268 MB) 57 us, 4.7 TB/s.  What is left is the
+// start of the pipeline, the join and the row-by-row epilogue.
+//
 // Waits are bounded as in linear_tc.cu.
 #include <stdio.h>
 #include "linear_epilogue.cuh"

@@ -22,6 +22,12 @@
 // operands in the weights' gradient) are loaded as MN-major tiles: boxes of 64 columns x 64
 // reduction rows, no transposed copies.
 //
+// Measured on a B200 (cuBLAS, plain product, beside it): 8192 x 8192 x 8192 bf16 693 us, 1586 TFLOP/s
+// (1752); 8192 x 2048 -> 8192 181 us, 1517 (1608), with gelu, residual and stored z 246 us; 16384 x
+// 1024 -> 1024 37 us, 932 (860); 8192 x 8192 -> 4096 e4m3 198 us, 2.8 PFLOP/s.  Tensor pipe active
+// 87 % in the input's gradient; a stage of the 256 x 256 pair tile moves 128 bytes a cycle through shared
+// memory, so operand traffic and MMAs are balanced, and long runs meet the power limit.
+//
 // Every mbarrier wait is bounded in time: on expiry the CTA raises a flag that ends all its loops,
 // sets the status word, gives its copies in flight a bounded time to land, frees its tensor memory
 // and returns.

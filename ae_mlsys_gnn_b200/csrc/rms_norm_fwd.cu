@@ -5,7 +5,15 @@
 //
 // Bound by HBM: x and residual are read once, y (or q) and h written once; the row stays in
 // registers between the sum of squares and the scaling.  y comes from the unrounded fp32 h; the
-// only roundings are those of the stored h, y and q.
+// only roundings are those of the stored h, y and q.  One group of threads a row and many CTAs:
+// walking rows with the next one's loads ahead, as the gradient does, measured slower here (16381 x
+// 2048 bf16: 64 against 47 us).
+//
+// Measured on a B200 (bytes of the arrays over event time): 16381 x 2048 bf16 with residual 47 us,
+// 5.7 TB/s = 0.87 of the copy bandwidth; 232965 x 256 fp32 78 us, 6.1 TB/s; 232965 x 602 fp32, whose rows
+// allow 8-byte accesses only, 268 us, 4.2 TB/s; e4m3 output, 16384 x 4096, 103 us, 4.6 TB/s, where the
+// conversions show (SM busy 0.78).  Rows of odd 16-bit widths move 2 bytes an access: 16384 x 4097
+// bf16 350 us.
 #include <cuda_fp8.h>
 #include <stdio.h>
 #include <type_traits>
