@@ -12,6 +12,10 @@
 // and 128 rows of output; its rate is not what bounds this shape.)
 // fp32: multiply-adds, lanes along the reduction axis, 4 or 8 rows a CTA (the row groups beyond the
 // first find W in L2).
+//
+// Measured on a B200 (event time, of which about 6 us are the events): 1 x 4096 -> 8192 bf16 (67 MB)
+// 18.4 us, e4m3 14.3 us, fp32 30.7 us; 1 x 28672 -> 8192 bf16 (470 MB) 82 us, 5.7 TB/s = 0.88 of the
+// copy bandwidth; 1 x 512 -> 512 bf16 at the floor of a launch.
 #include <stdio.h>
 #include "common.cuh"
 #include "linear_epilogue.cuh"

@@ -2,9 +2,9 @@
 // bytes of W.
 //
 // W is the 128-row operand of the tcgen05 MMA and the few rows of x are its N side, so a stage of the
-// TMA pipeline is 128 rows of W and only as many rows of x as there are (padded to 16, 32 or
-// 64), and two CTAs of an SM keep up to 192 KB of W in flight.  One CTA computes 128 columns of the output for
-// all rows; where N / 128 leaves SMs idle, a cluster of CTAs divides the reduction axis and its partial
+// TMA pipeline is 128 rows of W and only as many rows of x as there are (padded to 16, 32 or 64), and
+// two CTAs of an SM keep up to 192 KB of W in flight.  One CTA computes 128 columns of the output for all
+// rows; where N / 128 leaves SMs idle, a cluster of CTAs divides the reduction axis and its partial
 // sums meet in distributed shared memory, added in a fixed order.  In the accumulator a lane of
 // tensor memory is a column of the output: consecutive lanes store consecutive columns, bias and the
 // weights' scale are one value per thread.
@@ -24,7 +24,7 @@ namespace {
 constexpr int BM = 128;  // rows of W per CTA
 constexpr int kATile = BM * kStageK;
 constexpr int kThreads = 32 * 6;  // TMA, MMA, four epilogue warps
-constexpr int kMaxStages = 10;
+constexpr int kMaxStages = 6;
 constexpr int kHalfSm = 114 * 1024;  // shared memory of a CTA when two share an SM
 constexpr int kNumBars = 2 * kMaxStages + 1;
 constexpr int kBarBytes = (8 * kNumBars + 16 + 127) / 128 * 128;
