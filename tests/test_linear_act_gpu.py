@@ -413,6 +413,83 @@ def test_streams_graphs_and_scratch(cuda):
     assert torch.equal(got[0][0], step(*sets[0])[0])
 
 
+def test_two_streams_at_once(cuda):
+    """Calls of every kernel on two streams at the same time give what they give alone."""
+    from ae_mlsys_gnn_b200.operators import dense
+    from ae_mlsys_gnn_b200.operators.linear_act import linear_act, linear_act_fp8
+
+    gen = torch.Generator().manual_seed(12)
+    rnd = lambda *s: torch.randn(*s, generator=gen).to(cuda)
+    calls = []
+    for m in (3, 30, 60, 200, 1500):
+        x, w, r = rnd(m, 1024).bfloat16(), (rnd(1000, 1024) / 32).bfloat16(), rnd(m, 1000).bfloat16()
+        x8, xs = to_8_bits(rnd(m, 1024))
+        w8, ws = to_8_bits(rnd(1000, 1024) / 32)
+        calls.append(lambda x=x, w=w, r=r: linear_act(x, w, None, "gelu", r))
+        calls.append(lambda x=x.float(), w=w.float(): linear_act(x, w, None, "silu"))
+        calls.append(lambda x8=x8, xs=xs, w8=w8, ws=ws: linear_act_fp8(x8, xs, w8, ws))
+    want = [f() for f in calls]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = {s: [] for s in streams}
+    for _ in range(6):
+        for f in calls:
+            for s in streams:
+                with torch.cuda.stream(s):
+                    got[s].append(f())
+    torch.cuda.synchronize()
+    dense.check_status()
+    for s in streams:
+        for i, y in enumerate(got[s]):
+            assert torch.equal(y, want[i % len(calls)])
+
+
+def test_training_step_as_one_graph(cuda):
+    """A block of the operators with its optimizer as one captured step: the parameters after replays
+    are those of the same steps run eagerly."""
+    from ae_mlsys_gnn_b200.graphed import GraphedStep
+    from ae_mlsys_gnn_b200.operators import dense
+    from ae_mlsys_gnn_b200.operators.experts import expert_combine, expert_dispatch, expert_sort
+    from ae_mlsys_gnn_b200.operators.linear_act import linear_act
+    from ae_mlsys_gnn_b200.operators.rms_norm import add_rms_norm
+
+    gen = torch.Generator().manual_seed(21)
+    rnd = lambda *s: torch.randn(*s, generator=gen).to(cuda)
+    x, res, target = rnd(300, 64), rnd(300, 64), rnd(300, 64)
+    ids = torch.stack([torch.randperm(6, generator=gen)[:2] for _ in range(300)]).to(cuda)
+    probs = torch.full((300, 2), 0.5, device=cuda)
+    start = [torch.ones(64, device=cuda), rnd(96, 64) / 8, torch.zeros(96, device=cuda), rnd(64, 96) / 10]
+
+    def build():
+        params = [p.clone().requires_grad_(True) for p in start]
+        opt = torch.optim.SGD(params, lr=0.05)
+
+        def step():
+            opt.zero_grad(set_to_none=True)
+            y, h = add_rms_norm(x, params[0], res)
+            order = expert_sort(ids, 6)
+            f = linear_act(linear_act(expert_dispatch(y, order), params[1], params[2], "gelu"), params[3])
+            loss = (expert_combine(f, probs, order) + h - target).square().mean()
+            loss.backward()
+            opt.step()
+            return loss.detach()
+
+        return params, step
+
+    dense._status_word(cuda)
+    eager, step = build()
+    losses = [float(step()) for _ in range(7)]
+    captured, step = build()
+    graphed = GraphedStep(step, warmup=3)  # capturing runs nothing: three steps so far
+    for k in range(4):
+        graphed.replay()
+    torch.cuda.synchronize()
+    dense.check_status()
+    for a, b in zip(captured, eager):
+        assert torch.equal(a, b)
+    assert float(graphed.result) == losses[-1]
+
+
 def test_refusals(cuda):
     from ae_mlsys_gnn_b200.operators.linear_act import linear_act, linear_act_fp8
 
