@@ -32,6 +32,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include <stdlib.h>
+#include <type_traits>
 #include "../../include/gnn_b200.h"
 #include "common.cuh"
 #include "activation.cuh"
@@ -100,8 +101,14 @@ struct Params {
   float* score_l;
   float* score_r;
   int heads, head_w;
-  GemmFinish fin;  // read by the FINISH instantiation only
 };
+// With the epilogue of a linear layer.  Apart from Params, whose size alone changes the plain kernel's
+// registers (260 against 184 bytes of spills, 1 % of the weight gradient's time).
+struct FinishParams : Params {
+  GemmFinish fin;
+};
+template <bool FINISH>
+using KernelParams = std::conditional_t<FINISH, FinishParams, Params>;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -254,7 +261,7 @@ template <int BN, bool FINISH>
 __global__ void __launch_bounds__(Roles<FINISH>::kThreads, 1)
 gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_a1,
                        const __grid_constant__ CUtensorMap map_b0, const __grid_constant__ CUtensorMap map_b1,
-                       Params p) {
+                       KernelParams<FINISH> p) {
   constexpr int kStages = Geom<BN, FINISH>::kStages;
   constexpr int kStageBytes = Geom<BN, FINISH>::kStageBytes;
   constexpr int kBTileBytes = Geom<BN, FINISH>::kBTileBytes;
@@ -525,59 +532,61 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_
             }
             __syncwarp();  // the block is rewritten by the next chunk
           } else if (FINISH && last) {
-            // rows that are not whole 16-byte units: through the staging block as above, then a row at a
-            // time with neighbouring columns on neighbouring lanes
-            float4* const stg = epi_stage + (lg + 4 * part) * 256;
+            if constexpr (FINISH) {
+              // rows that are not whole 16-byte units: through the staging block as above, then a row at a
+              // time with neighbouring columns on neighbouring lanes
+              float4* const stg = epi_stage + (lg + 4 * part) * 256;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              stg[lane * 8 + (j ^ (lane & 7))] =
-                  make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]),
-                              __uint_as_float(r[4 * j + 3]));
-            __syncwarp();
-            const float* const flat = reinterpret_cast<const float*>(stg);
-            const int top = t.m0 + lg * 32, rows = min(32, p.M - top), col = col0 + lane;
-            const int unit = lane >> 2, word = lane & 3;
-            if (col < p.N) {
-              int64_t at = (int64_t)top * p.ldc + col;
-              if (!p.fin.bias && !p.fin.z && !p.fin.act && !p.fin.residual) {
-                if (rows == 32) {
+              for (int j = 0; j < 8; ++j)
+                stg[lane * 8 + (j ^ (lane & 7))] =
+                    make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]),
+                                __uint_as_float(r[4 * j + 3]));
+              __syncwarp();
+              const float* const flat = reinterpret_cast<const float*>(stg);
+              const int top = t.m0 + lg * 32, rows = min(32, p.M - top), col = col0 + lane;
+              const int unit = lane >> 2, word = lane & 3;
+              if (col < p.N) {
+                int64_t at = (int64_t)top * p.ldc + col;
+                if (!p.fin.bias && !p.fin.z && !p.fin.act && !p.fin.residual) {
+                  if (rows == 32) {
 #pragma unroll
-                  for (int r0 = 0; r0 < 32; r0 += 8) {
-                    float v[8];
+                    for (int r0 = 0; r0 < 32; r0 += 8) {
+                      float v[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = flat[((r0 + i) * 8 + (unit ^ i)) * 4 + word];
+                      for (int i = 0; i < 8; ++i) v[i] = flat[((r0 + i) * 8 + (unit ^ i)) * 4 + word];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) Cout[at + i * p.ldc] = v[i];
-                    at += 8 * p.ldc;
+                      for (int i = 0; i < 8; ++i) Cout[at + i * p.ldc] = v[i];
+                      at += 8 * p.ldc;
+                    }
+                  } else {
+#pragma unroll 1
+                    for (int rr = 0; rr < rows; ++rr, at += p.ldc) Cout[at] = flat[(rr * 8 + (unit ^ (rr & 7))) * 4 + word];
                   }
                 } else {
+                  const GemmFinish& f = p.fin;
+                  const float bias = f.bias ? __ldg(f.bias + col) : 0.f;
 #pragma unroll 1
-                  for (int rr = 0; rr < rows; ++rr, at += p.ldc) Cout[at] = flat[(rr * 8 + (unit ^ (rr & 7))) * 4 + word];
-                }
-              } else {
-                const GemmFinish& f = p.fin;
-                const float bias = f.bias ? __ldg(f.bias + col) : 0.f;
-#pragma unroll 1
-                for (int r0 = 0; r0 < rows; r0 += 8, at += 8 * p.ldc) {
-                  float v[8], res[8];
+                  for (int r0 = 0; r0 < rows; r0 += 8, at += 8 * p.ldc) {
+                    float v[8], res[8];
 #pragma unroll
-                  for (int i = 0; i < 8; ++i) {
-                    v[i] = flat[((r0 + i) * 8 + (unit ^ i)) * 4 + word] + bias;
-                    res[i] = f.residual && r0 + i < rows ? __ldg(f.residual + at + i * p.ldc) : 0.f;
-                  }
-                  if (f.z) {
+                    for (int i = 0; i < 8; ++i) {
+                      v[i] = flat[((r0 + i) * 8 + (unit ^ i)) * 4 + word] + bias;
+                      res[i] = f.residual && r0 + i < rows ? __ldg(f.residual + at + i * p.ldc) : 0.f;
+                    }
+                    if (f.z) {
+#pragma unroll
+                      for (int i = 0; i < 8; ++i)
+                        if (r0 + i < rows) f.z[at + i * p.ldc] = v[i];
+                    }
+                    apply_act<true>(v, f.act, f.slope);
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                      if (r0 + i < rows) f.z[at + i * p.ldc] = v[i];
+                      if (r0 + i < rows) Cout[at + i * p.ldc] = v[i] + res[i];
                   }
-                  apply_act<true>(v, f.act, f.slope);
-#pragma unroll
-                  for (int i = 0; i < 8; ++i)
-                    if (r0 + i < rows) Cout[at + i * p.ldc] = v[i] + res[i];
                 }
               }
+              __syncwarp();  // the block is rewritten by the next chunk
             }
-            __syncwarp();  // the block is rewritten by the next chunk
           } else if (last && row < p.M) {
             float* crow = Cout + (size_t)row * p.ldc + col0;
             const int ncols = min(32, p.N - col0);
@@ -695,7 +704,7 @@ bool encode_operand(const GemmOperand& o, int64_t K, CUtensorMap* m0, CUtensorMa
 
 template <int BN, bool FINISH>
 int launch_instance(const CUtensorMap& ma0, const CUtensorMap& ma1, const CUtensorMap& mb0, const CUtensorMap& mb1,
-                    Params p, int64_t b_rows, int splits, cudaStream_t stream) {
+                    KernelParams<FINISH> p, int64_t b_rows, int splits, cudaStream_t stream) {
   static bool attr_set = false;  // per process and instantiation; the attribute is per device
   static int attr_dev = -1;
   int dev = 0;
@@ -767,8 +776,10 @@ int launch_gemm_persistent(const GemmOperand& a, const GemmOperand& b, int64_t K
     return GNN_ERR_CUDA;
   }
   if (finish) {
-    p.fin = *finish;
-    return launch_instance<128, true>(ma0, ma1, mb0, mb1, p, b.rows, splits, stream);
+    FinishParams f;
+    static_cast<Params&>(f) = p;
+    f.fin = *finish;
+    return launch_instance<128, true>(ma0, ma1, mb0, mb1, f, b.rows, splits, stream);
   }
   return wide ? launch_instance<256, false>(ma0, ma1, mb0, mb1, p, b.rows, splits, stream)
               : launch_instance<128, false>(ma0, ma1, mb0, mb1, p, b.rows, splits, stream);
