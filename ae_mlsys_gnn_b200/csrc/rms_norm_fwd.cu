@@ -11,9 +11,9 @@
 //
 // Measured on a B200 (bytes of the arrays over event time): 16381 x 2048 bf16 with residual 47 us,
 // 5.7 TB/s = 0.87 of the copy bandwidth; 232965 x 256 fp32 78 us, 6.1 TB/s; 232965 x 602 fp32, whose rows
-// allow 8-byte accesses only, 268 us, 4.2 TB/s; e4m3 output, 16384 x 4096, 103 us, 4.6 TB/s, where the
+// allow 8-byte accesses only, 230 us, 4.9 TB/s; e4m3 output, 16384 x 4096, 103 us, 4.6 TB/s, where the
 // conversions show (SM busy 0.78).  Rows of odd 16-bit widths move 2 bytes an access: 16384 x 4097
-// bf16 350 us.
+// bf16 206 us.
 #include <cuda_fp8.h>
 #include <stdio.h>
 #include <type_traits>
@@ -60,12 +60,13 @@ __global__ void __launch_bounds__(MAXT, MAXT == 512 && sizeof(T) * VEC * NV <= 1
   P a[NV], r[NV];
   const P* xr = reinterpret_cast<const P*>(static_cast<const T*>(p.x) + (live ? row : 0) * p.d);
   const P* rr = reinterpret_cast<const P*>(static_cast<const T*>(p.residual) + (live ? row : 0) * p.d);
+  // no condition around the loads (the compiler would move them to their uses): what lies behind the row
+  // is its last piece again and is not used
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (live && t + G * i < nvec) {
-      a[i] = load_pack(xr + t + G * i);
-      if (p.residual) r[i] = load_pack(rr + t + G * i);
-    }
+  for (int i = 0; i < NV; ++i) {
+    a[i] = load_pack(xr + min(t + G * i, nvec - 1));
+    if (p.residual) r[i] = load_pack(rr + min(t + G * i, nvec - 1));
+  }
 
   float v[NV][VEC];
   float sq = 0.f;
