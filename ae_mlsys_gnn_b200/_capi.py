@@ -122,6 +122,9 @@ PROTOTYPES = {
     "gnn_linear_dgrad": [_PTR, _I64, _PTR, _I64, _INT, _PTR, _I64, _I64, _I64, _PTR, _SZ, _PTR, _PTR],
     "gnn_linear_wgrad_workspace_bytes": [_I64, _I64, _I64, _INT, _SZP],
     "gnn_linear_wgrad": [_PTR, _I64, _PTR, _I64, _INT, _PTR, _I64, _I64, _I64, _PTR, _SZ, _PTR, _PTR],
+    "gnn_linear_bwd_workspace_bytes": [_I64, _I64, _I64, _INT, _INT, _SZP],
+    "gnn_linear_bwd": [_PTR, _PTR, _INT, _F32, _PTR, _I64, _PTR, _I64, _INT, _INT, _PTR, _PTR, _PTR, _I64, _I64, _I64,
+                       _PTR, _SZ, _PTR, _PTR],
     "gnn_pad_rows": [_PTR, _INT, _I64, _I64, _PTR, _I64, _PTR],
     "gnn_expert_sort_workspace_bytes": [_I64, _INT, _SZP],
     "gnn_expert_sort": [_PTR, _INT, _I64, _INT, _PTR, _PTR, _PTR, _SZ, _PTR],
@@ -193,7 +196,7 @@ KERNELS_PER_CALL = {
     "gnn_edge_softmax_fwd": 1, "gnn_edge_softmax_bwd": 1, "gnn_knn_graph": 1, "gnn_halo_push": 1, "gnn_halo_push_ranges": 1,
     "gnn_rms_norm_fwd": 1, "gnn_rms_norm_fp8": 1, "gnn_rms_norm_bwd": 2,
     # product (+ weight split for fp32, + sum of the ranges when the reduction is split)
-    "gnn_linear_fwd": 1, "gnn_linear_act_bwd": 2, "gnn_linear_dgrad": 1, "gnn_linear_wgrad": 2, "gnn_pad_rows": 1,
+    "gnn_linear_fwd": 1, "gnn_linear_act_bwd": 2, "gnn_linear_dgrad": 1, "gnn_linear_wgrad": 2, "gnn_linear_bwd": 5, "gnn_pad_rows": 1,
     # count + place (one kernel up to 1024 pairs)
     "gnn_expert_sort": 2, "gnn_expert_dispatch": 1, "gnn_expert_combine": 1, "gnn_expert_combine_bwd": 1,
 }

@@ -379,6 +379,53 @@ extern "C" int gnn_linear_wgrad(const void* gz, int64_t ldg, const void* x, int6
   return launch_linear_tc(a, b, dtype, N, K, M, ep, workspace, workspace_bytes, status, stream, what);
 }
 
+// The three steps of a gradient in one call: small layers are bound by the host.
+extern "C" int gnn_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int own_gz, size_t* bytes) {
+  if (!bytes || M < 0 || N < 1 || K < 1 || !is_float(dtype))
+    return fail(GNN_ERR_INVALID_ARG, "gnn_linear_bwd_workspace_bytes", "bad argument");
+  const int64_t per = 16 / dtype_bytes(dtype), ldz = (N + per - 1) / per * per;
+  size_t act = 0, dx = 0, dw = 0;
+  gnn_linear_act_bwd_workspace_bytes(M, N, ldz, &act);
+  gnn_linear_dgrad_workspace_bytes(M, N, K, dtype, &dx);
+  gnn_linear_wgrad_workspace_bytes(M, N, K, dtype, &dw);
+  const size_t most = act > dx ? (act > dw ? act : dw) : (dx > dw ? dx : dw);
+  *bytes = most + 256 + (own_gz ? ((size_t)M * ldz * dtype_bytes(dtype) + 511) / 256 * 256 : 0);
+  return GNN_OK;
+}
+
+extern "C" int gnn_linear_bwd(const void* grad_y, const void* z, int act, float slope, const void* x, int64_t ldx,
+                              const void* w, int64_t ldw, int dtype, int own_gz, void* grad_x, void* grad_w, void* grad_b,
+                              int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes, int* status,
+                              cudaStream_t stream) {
+  const char* const what = "gnn_linear_bwd";
+  if (int rc = check_sizes(what, M, N, K)) return rc;
+  if (!is_float(dtype)) return fail(GNN_ERR_UNSUPPORTED, what, "operands are fp32, bf16 or fp16");
+  if (act && !own_gz && (grad_x || grad_w)) return fail(GNN_ERR_INVALID_ARG, what, "an activation needs own_gz");
+  size_t need = 0;
+  gnn_linear_bwd_workspace_bytes(M, N, K, dtype, own_gz, &need);
+  if (!workspace || workspace_bytes < need) return fail(GNN_ERR_WORKSPACE, what, "workspace too small");
+  const int64_t per = 16 / dtype_bytes(dtype);
+  uintptr_t at = ((uintptr_t)workspace + 255) & ~(uintptr_t)255;
+  const void* gz = grad_y;
+  int64_t ldg = N;
+  void* own = nullptr;
+  if (own_gz) {
+    gz = own = (void*)at;
+    ldg = (N + per - 1) / per * per;
+    at = (at + (size_t)M * ldg * dtype_bytes(dtype) + 255) & ~(uintptr_t)255;
+  }
+  // the steps follow each other on the stream, so they share what is left
+  void* const rest = (void*)at;
+  const size_t left = (uintptr_t)workspace + workspace_bytes - at;
+  if (own || grad_b)
+    if (int rc = gnn_linear_act_bwd(grad_y, z, act, slope, dtype, M, N, own, ldg, grad_b, rest, left, stream)) return rc;
+  if (grad_x)
+    if (int rc = gnn_linear_dgrad(gz, ldg, w, ldw, dtype, grad_x, M, N, K, rest, left, status, stream)) return rc;
+  if (grad_w)
+    if (int rc = gnn_linear_wgrad(gz, ldg, x, ldx, dtype, grad_w, M, N, K, rest, left, status, stream)) return rc;
+  return GNN_OK;
+}
+
 extern "C" int gnn_pad_rows(const void* src, int element_bytes, int64_t rows, int64_t cols, void* dst, int64_t ld,
                             cudaStream_t stream) {
   const char* const what = "gnn_pad_rows";

@@ -65,7 +65,7 @@ __device__ __forceinline__ void load_weight(const void* w, int w_f32, int64_t co
 // Elements per thread.  Many threads with few elements each keep more loads in flight, but the wide
 // rows of the forward pass run better as two CTAs of 512 threads an SM than as one of 1024 (8192 x
 // 8192 bf16: 106 against 166 us); rows of narrow accesses (16384 x 4098: 166 against 217 us) and the
-// gradient (189 against 273 us), whose registers do not last for 16 elements, stay at 8 until 1024
+// gradient (8192 x 8192: 189 against 273 us), whose registers do not last for 16 elements, stay at 8 until 1024
 // threads hold the row.  `mid`: the kernel has a form with 16.
 inline int norm_ept(int64_t d, bool mid) {
   if (mid) return d <= 4096 ? 8 : d <= 8192 ? 16 : 32;

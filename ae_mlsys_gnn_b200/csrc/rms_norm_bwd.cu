@@ -10,7 +10,7 @@
 //
 // Measured on a B200: 16381 x 2048 bf16 with residual 73 us, 3.7 TB/s = 0.56 of the copy bandwidth
 // (about 30 instructions an element and a reduction per row at three CTAs an SM bound it, DRAM is
-// a third busy); 232965 x 256 fp32 125 us, 5.7 TB/s; 232965 x 602 fp32 373 us, 4.5 TB/s.
+// a third busy); 232965 x 256 fp32 120 us, 6.0 TB/s; 232965 x 602 fp32 376 us, 4.5 TB/s.
 #include <algorithm>
 #include <type_traits>
 #include "rms_norm.cuh"

@@ -94,6 +94,17 @@ class _LinearAct(torch.autograd.Function):
         per = 16 // x.element_size()
         ldz = -(-N // per) * per
         products = (need_x or need_w) and M > 0
+        if products and (code != 0 or (N % 4 == 0 and K % 4 == 0)):  # one call for all steps
+            own = int(act != 0 or ldz != N or gy.data_ptr() % 16 != 0)
+            gx = torch.empty((M, K), dtype=dt, device=dev) if need_x else None
+            gw = torch.empty((N, K), dtype=dt, device=dev) if need_w else None
+            gb = torch.empty(N, dtype=dt, device=dev) if need_b else None
+            scratch, nbytes = capi.scratch("gnn_linear_bwd_workspace_bytes", dev, M, N, K, code, own)
+            ptr = capi.ptr
+            capi.launch(dev, "gnn_linear_bwd", gy.data_ptr(), ptr(z), act, slope, x.data_ptr(), x.shape[1], w.data_ptr(),
+                        w.shape[1], code, own, ptr(gx), ptr(gw), ptr(gb), M, N, K, scratch.data_ptr(), nbytes,
+                        _status(dev).data_ptr())
+            return gx, gw, gb, (gy if need_r else None), None, None
         gz = gy
         own_gz = products and (act != 0 or ldz != N or gy.data_ptr() % 16 != 0)
         if own_gz:

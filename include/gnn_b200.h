@@ -483,6 +483,15 @@ int gnn_rms_norm_bwd(const void* grad_y, const void* grad_h, const void* h, cons
                      int dtype, int weight_dtype, int64_t n, int64_t d, void* grad_x, void* grad_w, void* workspace,
                      size_t workspace_bytes, cudaStream_t stream);
 
+/* The steps of the gradient above in one call (any of grad_x, grad_w, grad_b may be NULL).  own_gz != 0:
+ * gz is formed in the workspace, rows a multiple of 16 bytes apart; needed with an activation, and
+ * where grad_y's rows do not start on 16-byte boundaries.  fp32: N and K multiples of 4. */
+int gnn_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int own_gz, size_t* bytes);
+int gnn_linear_bwd(const void* grad_y, const void* z, int act, float slope, const void* x, int64_t ldx,
+                   const void* w, int64_t ldw, int dtype, int own_gz, void* grad_x, void* grad_w, void* grad_b,
+                   int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes, int* status,
+                   cudaStream_t stream);
+
 /* Rows between token order and expert order.  Every token has k choices (pairs, numbered t*k + j);
  * a pair whose expert is not one of 0..n_experts-1 (a padding token's -1) goes nowhere.
  * gnn_expert_sort: stable counting sort of the pairs by expert.  offsets [n_experts+1]: first row

@@ -110,6 +110,20 @@ def test_linear_c_refusals():
         assert f(dt=F32) == -3 and f(dt=F32, ldg=12) == -4
 
 
+def test_linear_bwd_c_refusals():
+    from ae_mlsys_gnn_b200 import _capi
+
+    lib = _capi.lib()
+    need = ctypes.c_size_t(0)
+    size = lambda M=100, N=64, dt=1, own=1: lib.gnn_linear_bwd_workspace_bytes(M, N, 64, dt, own, ctypes.byref(need))
+    assert size() == 0 and need.value >= 100 * 64 * 2
+    assert size(N=0) == -1 and size(M=-1) == -1 and size(dt=3) == -1 and size() == 0
+    bwd = lambda act=4, own=1, ws=ONE, nb=need.value, dt=1, M=100: lib.gnn_linear_bwd(
+        ONE, ONE, act, 0.2, ONE, 64, ONE, 64, dt, own, ONE, ONE, ONE, M, 64, 64, ws, nb, ONE, None)
+    assert bwd(own=0) == -1 and bwd(ws=None) == -3 and bwd(nb=need.value - 1) == -3
+    assert bwd(dt=3) == -4 and bwd(M=-1) == -1
+
+
 def test_pad_rows_c_refusals():
     from ae_mlsys_gnn_b200 import _capi
 
