@@ -2,7 +2,7 @@
 //
 // Bound by the bytes of W, each of which is used for M multiply-adds only: the kernel's whole task is
 // to keep enough loads in flight on every SM.  Columns of the output (rows of W) are spread over the
-// CTAs 16 or 32 at a time and the reduction axis over a CTA's eight warps and over the CTAs of a
+// CTAs 16 at a time and the reduction axis over a CTA's eight warps and over the CTAs of a
 // cluster; the partial sums meet in (distributed) shared memory and are added in a fixed order.
 //
 // 16-bit and 8-bit: warp-level MMAs with 16 rows of W as the 16-row operand and 8 rows of x as the
@@ -113,9 +113,10 @@ __device__ __forceinline__ void join_and_finish(const LinearEpilogue& ep, float*
   cluster_sync();  // nobody leaves while its sums are being read
 }
 
-// NT tiles of 16 columns, MG groups of 8 rows; U pieces of 64 bytes of every row are requested at once.
-template <int KIND, int MG, int NT, int U>
+// 16 columns and 8 rows a CTA; U pieces of 64 bytes of every row are requested at once.
+template <int KIND>
 __global__ void __launch_bounds__(32 * kWarps, 4) few_mma_kernel(const FewParams p) {
+  constexpr int MG = 1, NT = 1, U = 4;  // groups of 8 rows, tiles of 16 columns
   __shared__ float parts[kWarps * MG * 8 * NT * 16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int col0 = blockIdx.x * (16 * NT);
@@ -255,7 +256,7 @@ bool launch(Kernel kernel, int64_t col_ctas, int cluster, const FewParams& p, cu
 template <int KIND>
 void launch_kind(const FewParams& p, cudaStream_t stream) {
   const int64_t ctas = (p.N + 15) / 16;
-  launch(few_mma_kernel<KIND, 1, 1, 4>, ctas, cluster_for(ctas, (p.row_bytes + 255) / 256), p, stream);
+  launch(few_mma_kernel<KIND>, ctas, cluster_for(ctas, (p.row_bytes + 255) / 256), p, stream);
 }
 
 }  // namespace

@@ -31,7 +31,8 @@ def _status(dev):
     if t is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the first matrix product on a device must run before a graph is captured")
-        t = dense._status_word(dev)
+        with torch.inference_mode(False):  # it is also reset outside of inference mode
+            t = dense._status_word(dev)
     return t
 
 

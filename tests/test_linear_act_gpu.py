@@ -254,6 +254,27 @@ def test_leading_dimensions_strides_and_alignment(cuda):
             assert bool(torch.isfinite(a).all())
 
 
+def test_8_bit_operands_strided_shifted_and_empty(cuda):
+    from ae_mlsys_gnn_b200.operators.linear_act import linear_act_fp8
+
+    gen = torch.Generator().manual_seed(14)
+    for m, k in ((40, 96), (40, 100), (300, 96)):
+        x8, xs = to_8_bits(torch.randn(m, k, generator=gen).to(cuda))
+        w8, ws = to_8_bits(torch.randn(72, k, generator=gen).to(cuda))
+        y = linear_act_fp8(x8, xs, w8, ws)
+        wide = torch.zeros(m, k + 30, device=cuda).to(torch.float8_e4m3fn)
+        wide[:, 7:7 + k] = x8
+        assert torch.equal(linear_act_fp8(wide[:, 7:7 + k], xs, w8, ws), y)
+        flat = torch.zeros(m * k + 3, device=cuda).to(torch.float8_e4m3fn)
+        shifted = flat[3:].view(m, k)
+        shifted.copy_(x8)
+        assert torch.equal(linear_act_fp8(shifted, xs, w8, ws), y)
+        assert torch.equal(linear_act_fp8(x8.view(4, m // 4, k), xs, w8, ws).view(m, 72), y)
+        assert linear_act_fp8(x8[:0], xs[:0], w8, ws).shape == (0, 72)
+        with torch.inference_mode():
+            assert torch.equal(linear_act_fp8(x8, xs, w8, ws), y)
+
+
 def test_empty_and_special_values(cuda):
     from ae_mlsys_gnn_b200.operators.linear_act import linear_act
 
